@@ -65,6 +65,18 @@ SIGNATURES = {
     "cvb_fits_shared": (_c.c_int, [_c.c_int, _c.c_int]),
     "cvb_cross_spectrum": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int] * 7 + [_c.c_void_p]),
     "cvb_cross_spectrum_supported": (_c.c_int, [_c.c_int, _c.c_int]),
+    "cvb_residual_norm_fwd": (_c.c_int, [_c.c_void_p]),
+    "cvb_residual_norm_workspace_bytes": (_c.c_size_t, [_c.c_int, _c.c_longlong, _c.c_int]),
+    "cvb_residual_norm_bwd": (_c.c_int, [_c.c_void_p]),
+    "cvb_clip_workspace_bytes": (_c.c_size_t, [_c.c_int]),
+    "cvb_clip_by_norm": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_int, _c.c_double, _c.c_int] + [_c.c_void_p] * 2 +
+                         [_c.c_size_t, _c.c_void_p]),
+    "cvb_quantize_tokens": (_c.c_int, [_c.c_void_p] * 3 + [_c.c_longlong] * 2 + [_c.c_int, _c.c_longlong, _c.c_int, _c.c_int, _c.c_void_p]),
+    "cvb_int8_product": (_c.c_int, [_c.c_void_p, _c.c_longlong, _c.c_void_p, _c.c_void_p, _c.c_longlong] + [_c.c_void_p] * 3 +
+                         [_c.c_longlong] * 2 + [_c.c_int] * 4 + [_c.c_void_p]),
+    "cvb_pointwise_int8_workspace_bytes": (_c.c_size_t, [_c.c_longlong] * 2 + [_c.c_int] * 4),
+    "cvb_pointwise_int8": (_c.c_int, [_c.c_void_p] * 2 + [_c.c_longlong] + [_c.c_void_p] * 3 + [_c.c_longlong] * 2 + [_c.c_int] * 4 +
+                           [_c.c_void_p, _c.c_size_t, _c.c_void_p]),
     "cvb_tap_gradient": (_c.c_int, [_c.c_void_p] * 3 + [_c.c_int] * 7 + [_c.c_void_p]),
 }
 

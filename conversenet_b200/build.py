@@ -89,7 +89,8 @@ def _units():
     units = [("converse_b200", "converse_b200.cu", []), ("k_dynamic", "k_dynamic.cu", []),
              ("k_strip", "k_strip.cu", []), ("k_block", "k_block.cu", []), ("k_block_tc", "k_block_tc.cu", []), ("k_block_tc2", "k_block_tc2.cu", []),
              ("k_block_tc3", "k_block_tc3.cu", []), ("k_block_mlp", "k_block_mlp.cu", []), ("k_block_train", "k_block_train.cu", [])]
-    units += [("k_rp", "k_rp.cu", []), ("k_rp_rows", "k_rp_rows.cu", []), ("k_rp_bwd", "k_rp_bwd.cu", []), ("k_fix", "k_fix.cu", [])]
+    units += [("k_rp", "k_rp.cu", []), ("k_rp_rows", "k_rp_rows.cu", []), ("k_rp_bwd", "k_rp_bwd.cu", []), ("k_fix", "k_fix.cu", []),
+              ("k_seam", "k_seam.cu", []), ("k_clip", "k_clip.cu", []), ("k_int8", "k_int8.cu", [])]
     for name, io in (("f32", "float"), ("bf16", "__nv_bfloat16")):
         for unit in ("k_rp_cols", "k_rp_plane"):
             units.append(("%s_%s" % (unit, name), unit + ".cu", ["-DCVB_IO=" + io, "-DCVB_IO_NAME=" + name]))
@@ -144,7 +145,7 @@ def build_host(force=False):
     """The native host module next to this file; rebuilt when its source, the C ABI or torch changed."""
     cmd = _host_command()
     h = hashlib.sha1(" ".join(cmd).encode())
-    for path in (os.path.join(CSRC, "host.cpp"), os.path.join(HERE, "..", "include", "converse_b200.h")):
+    for path in (os.path.join(CSRC, "host.cpp"), os.path.join(CSRC, "host_ops.h"), os.path.join(HERE, "..", "include", "converse_b200.h")):
         h.update(open(path, "rb").read())
     stamp = os.path.join(OBJ, "host.stamp")
     if not force and os.path.exists(HOST) and os.path.exists(stamp) and open(stamp).read() == h.hexdigest():

@@ -5,6 +5,7 @@
 #include "cvb_plan.h"
 #include "cvb_block.cuh"
 #include "cvb_rp_plan.h"
+#include "cvb_seam.h"
 
 #include <algorithm>
 #include <cstdlib>
@@ -711,6 +712,124 @@ int cvb_block_post_fwd(const void* t, const void* x, void* out, const void* pack
   if (io_dtype != CVB_F32 && io_dtype != CVB_BF16) return CVB_ERR_BAD_ARGUMENT;
   return launch_block_mix(true, x, t, out, pack, ln_eps, B, HW, io_dtype, sm_count(), status_ptr(),
                           (cudaStream_t)stream);
+}
+
+// What both directions of the seam ask of their arguments; the kernels' parameters
+static int seam_params(const cvb_residual_norm_args& A, bool backward, seam::Params& P) {
+  if (!A.branch && !backward) return CVB_ERR_BAD_ARGUMENT;
+  if (A.B < 1 || A.HW < 1 || A.C < 1 || A.HW > (1ll << 40) / A.B) return CVB_ERR_BAD_ARGUMENT;
+  if (A.io_dtype != CVB_F32 && A.io_dtype != CVB_BF16) return CVB_ERR_BAD_ARGUMENT;
+  if (A.gate_kind < CVB_GATE_NONE || A.gate_kind > CVB_GATE_IMAGE || (A.gate_kind != CVB_GATE_NONE) != (A.gate != nullptr))
+    return CVB_ERR_BAD_ARGUMENT;
+  if ((A.post_b && !A.post_w) || (A.pre_b && !A.pre_w) || !(A.eps >= 0.f)) return CVB_ERR_BAD_ARGUMENT;
+  if (A.C > 16384) return CVB_ERR_TOO_LARGE;
+  memset(&P, 0, sizeof(P));
+  P.x = A.x; P.branch = A.branch; P.gate = A.gate; P.y = A.y; P.z = A.z;
+  P.scale = A.scale; P.post_w = A.post_w; P.post_b = A.post_b; P.pre_w = A.pre_w; P.pre_b = A.pre_b;
+  P.stats = A.stats;
+  P.B = A.B; P.HW = A.HW; P.tokens = A.B * A.HW; P.C = A.C;
+  P.first = !A.channels_last; P.rms = A.rms != 0; P.gate_kind = A.gate_kind; P.act = A.gate_act != 0; P.eps = A.eps;
+  // one pixel an image: the layouts are the same, and tokens side by side fill a warp
+  if (P.first && P.HW == 1) P.first = 0;
+  const long long blocks = P.first ? (P.HW + 31) / 32 * P.B : P.tokens;
+  if (blocks > 0x7fffffffll || (A.gate_kind == CVB_GATE_IMAGE && P.B > 0xffffffll)) return CVB_ERR_TOO_LARGE;
+  return seam::takes(P.C, P.first != 0, backward) ? CVB_OK : CVB_ERR_TOO_LARGE;
+}
+
+int cvb_residual_norm_fwd(const cvb_residual_norm_args* args) {
+  if (!args) return CVB_ERR_BAD_ARGUMENT;
+  seam::Params P;
+  const int rc = seam_params(*args, false, P);
+  if (rc != CVB_OK) return rc;
+  if (!P.x || !P.y || (P.pre_w && !P.z)) return CVB_ERR_BAD_ARGUMENT;
+  return seam::run_fwd(P, args->io_dtype, sm_count(), (cudaStream_t)args->stream);
+}
+
+size_t cvb_residual_norm_workspace_bytes(int C, long long B, int gate_kind) {
+  if (C < 1 || B < 1) return 0;
+  const size_t parts = seam::most_parts(C, B, gate_kind, sm_count());
+  return parts * (gate_kind == CVB_GATE_IMAGE ? (size_t)B : 1) * 4 * C * sizeof(float);
+}
+
+int cvb_residual_norm_bwd(const cvb_residual_norm_args* args) {
+  if (!args) return CVB_ERR_BAD_ARGUMENT;
+  const cvb_residual_norm_args& A = *args;
+  seam::Params P;
+  const int rc = seam_params(A, true, P);
+  if (rc != CVB_OK) return rc;
+  const bool sums = A.dscale || A.dpost_w || A.dpost_b || A.dpre_w || A.dpre_b || (A.dgate && A.gate_kind == CVB_GATE_IMAGE);
+  P.dy = A.dy; P.dz = A.dz; P.dx = A.dx; P.dbranch = A.dbranch; P.dgate = A.dgate;
+  P.dscale = A.dscale; P.dpost_w = A.dpost_w; P.dpost_b = A.dpost_b; P.dpre_w = A.dpre_w; P.dpre_b = A.dpre_b;
+  if ((!P.dy && !P.dz) || (P.dz && (!P.pre_w || !P.x || !P.branch)) || ((P.dz || P.post_w) && !P.stats)) return CVB_ERR_BAD_ARGUMENT;
+  if (!P.branch && (P.dbranch || P.dgate || P.dscale || P.dpost_w || P.dpost_b)) return CVB_ERR_BAD_ARGUMENT;
+  if (!P.dx && !P.dbranch && !P.dgate && !sums) return CVB_ERR_BAD_ARGUMENT;
+  if (sums) {
+    if (!A.workspace || A.workspace_bytes < cvb_residual_norm_workspace_bytes(A.C, A.B, A.gate_kind)) return CVB_ERR_WORKSPACE;
+    P.partial = (float*)A.workspace;
+  }
+  P.max_parts = seam::most_parts(A.C, A.B, A.gate_kind, sm_count());
+  return seam::run_bwd(P, A.io_dtype, sm_count(), (cudaStream_t)A.stream);
+}
+
+size_t cvb_clip_workspace_bytes(int count) { return clip_workspace(count, sm_count()); }
+
+int cvb_clip_by_norm(const cvb_span* spans, int count, int kind, double max_norm, int scale_them, float* norm,
+                     void* workspace, size_t workspace_bytes, void* stream) {
+  if (count < 0 || (count && !spans) || !norm || kind < 0 || kind > 2) return CVB_ERR_BAD_ARGUMENT;
+  if (scale_them && !(max_norm >= 0)) return CVB_ERR_BAD_ARGUMENT;
+  for (int i = 0; i < count; ++i) {
+    const cvb_span& s = spans[i];
+    if (s.n < 0 || s.n > (1ll << 45) || (s.in_type != CVB_F32 && s.in_type != CVB_BF16)) return CVB_ERR_BAD_ARGUMENT;
+    if (s.n && (!s.in || (size_t)s.in % (s.in_type == CVB_F32 ? 4 : 2))) return CVB_ERR_BAD_ARGUMENT;
+    if (!scale_them) continue;
+    if (s.out_type != CVB_F32 && s.out_type != CVB_BF16) return CVB_ERR_BAD_ARGUMENT;
+    if (s.n && (!s.out || (size_t)s.out % (s.out_type == CVB_F32 ? 4 : 2) || (s.in == s.out && s.in_type != s.out_type)))
+      return CVB_ERR_BAD_ARGUMENT;
+  }
+  if (!workspace || workspace_bytes < clip_workspace(count, sm_count())) return CVB_ERR_WORKSPACE;
+  return run_clip(spans, count, kind, max_norm, scale_them != 0, norm, workspace, sm_count(), (cudaStream_t)stream);
+}
+
+// Sizes that the 8-bit products share: tokens are rows of a tensor map
+static int check_int8(long long B, long long HW, int K, int io_dtype) {
+  if (B < 1 || HW < 1 || K < 1 || (io_dtype != CVB_F32 && io_dtype != CVB_BF16)) return CVB_ERR_BAD_ARGUMENT;
+  return K > 131072 || HW > 0x7fffff00ll / B ? CVB_ERR_TOO_LARGE : CVB_OK;
+}
+static bool int8_rows(const void* p, long long ld, int K) { return p && (size_t)p % 16 == 0 && ld % 16 == 0 && ld >= K; }
+
+int cvb_quantize_tokens(const void* x, signed char* q, float* scale, long long B, long long HW, int K, long long ldq,
+                        int channels_last, int io_dtype, void* stream) {
+  const int rc = check_int8(B, HW, K, io_dtype);
+  if (rc != CVB_OK) return rc;
+  if (!x || !scale || !int8_rows(q, ldq, K)) return CVB_ERR_BAD_ARGUMENT;
+  return i8::run_quantize(x, q, scale, B, HW, K, ldq, channels_last != 0, io_dtype, (cudaStream_t)stream);
+}
+
+int cvb_int8_product(const signed char* q, long long ldq, const float* scale, const signed char* w, long long ldw,
+                     const float* w_scale, const float* bias, void* out, long long B, long long HW, int K, int N,
+                     int channels_last, int io_dtype, void* stream) {
+  const int rc = check_int8(B, HW, K, io_dtype);
+  if (rc != CVB_OK) return rc;
+  if (!int8_rows(q, ldq, K) || !int8_rows(w, ldw, K) || !scale || !w_scale || !out || N < 1) return CVB_ERR_BAD_ARGUMENT;
+  return i8::run_product(q, ldq, scale, w, ldw, w_scale, bias, out, B, HW, K, N, channels_last != 0, io_dtype, sm_count(),
+                         status_ptr(), (cudaStream_t)stream);
+}
+
+size_t cvb_pointwise_int8_workspace_bytes(long long B, long long HW, int K, int N, int channels_last, int io_dtype) {
+  if (check_int8(B, HW, K, io_dtype) != CVB_OK || N < 1) return 0;
+  return i8::workspace(B, HW, K, N, channels_last != 0, io_dtype);
+}
+
+int cvb_pointwise_int8(const void* x, const signed char* w, long long ldw, const float* w_scale, const float* bias, void* out,
+                       long long B, long long HW, int K, int N, int channels_last, int io_dtype, void* workspace,
+                       size_t workspace_bytes, void* stream) {
+  const int rc = check_int8(B, HW, K, io_dtype);
+  if (rc != CVB_OK) return rc;
+  if (!x || !int8_rows(w, ldw, K) || !w_scale || !out || N < 1) return CVB_ERR_BAD_ARGUMENT;
+  const size_t need = i8::workspace(B, HW, K, N, channels_last != 0, io_dtype);
+  if (need && (!workspace || (size_t)workspace % 16 || workspace_bytes < need)) return CVB_ERR_WORKSPACE;
+  return i8::run_pointwise(x, w, ldw, w_scale, bias, out, B, HW, K, N, channels_last != 0, io_dtype, workspace, sm_count(),
+                           status_ptr(), (cudaStream_t)stream);
 }
 
 }  // extern "C"

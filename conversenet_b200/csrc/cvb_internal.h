@@ -115,6 +115,23 @@ size_t block_grad_workspace(int B, int HW, size_t conv_ws, int sms);
 int run_block_grad(const cvb_block_bwd_args& A, size_t conv_ws, int sms, int* status, cudaStream_t st,
                    int (*conv)(const cvb_block_bwd_args&, const float* gu, float* gt, void* ws, size_t bytes));
 
+// norm of many tensors, and the tensors scaled (k_clip.cu)
+size_t clip_workspace(int count, int sms);
+int run_clip(const cvb_span* spans, int count, int kind, double max_norm, bool scale, float* norm, void* workspace, int sms,
+             cudaStream_t st);
+
+// 1x1 products in 8-bit integers (k_int8.cu)
+namespace i8 {
+int run_quantize(const void* x, signed char* q, float* scale, long long B, long long HW, int K, long long ldq, bool last, int io,
+                 cudaStream_t st);
+int run_product(const signed char* q, long long ldq, const float* scale, const signed char* w, long long ldw, const float* w_scale,
+                const float* bias, void* out, long long B, long long HW, int K, int N, bool last, int io, int sms, int* status,
+                cudaStream_t st);
+size_t workspace(long long B, long long HW, int K, int N, bool last, int io);
+int run_pointwise(const void* x, const signed char* w, long long ldw, const float* w_scale, const float* bias, void* out,
+                  long long B, long long HW, int K, int N, bool last, int io, void* ws, int sms, int* status, cudaStream_t st);
+}  // namespace i8
+
 // Multi-pass kernels with a compile-time axis plan (k_strip2.cu, one object per registry line).
 struct StripParams;
 typedef int (*Strip2Launcher)(const StripParams& SP, int io_dtype, cudaStream_t st);

@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cstdlib>
 #include <cstring>
 #include <memory>
@@ -54,6 +55,15 @@ struct Api {
   decltype(&cvb_takes_planes) takes_planes = nullptr;
   decltype(&cvb_plane_workspace_bytes) plane_workspace_bytes = nullptr;
   decltype(&cvb_plane_fwd) plane_fwd = nullptr;
+  decltype(&cvb_residual_norm_fwd) residual_norm_fwd = nullptr;
+  decltype(&cvb_residual_norm_workspace_bytes) residual_norm_workspace = nullptr;
+  decltype(&cvb_residual_norm_bwd) residual_norm_bwd = nullptr;
+  decltype(&cvb_clip_workspace_bytes) clip_workspace = nullptr;
+  decltype(&cvb_clip_by_norm) clip_by_norm = nullptr;
+  decltype(&cvb_quantize_tokens) quantize_tokens = nullptr;
+  decltype(&cvb_int8_product) int8_product = nullptr;
+  decltype(&cvb_pointwise_int8_workspace_bytes) pointwise_int8_workspace = nullptr;
+  decltype(&cvb_pointwise_int8) pointwise_int8 = nullptr;
 } api;
 
 struct Failed : std::runtime_error { using std::runtime_error::runtime_error; };
@@ -571,12 +581,14 @@ PyObject* py_block_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+#include "host_ops.h"
+
 // init(address of each C ABI function in the order of `names`)
 PyObject* py_init(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    want(n, 30);
-    void* p[30];
-    for (int i = 0; i < 30; ++i) p[i] = PyLong_AsVoidPtr(a[i]);
+    want(n, 39);
+    void* p[39];
+    for (int i = 0; i < 39; ++i) p[i] = PyLong_AsVoidPtr(a[i]);
     int i = 0;
     auto set = [&](auto& f) { f = (std::decay_t<decltype(f)>)p[i++]; };
     set(api.strerror_); set(api.last_cuda_error); set(api.transfer_bytes); set(api.build_transfer); set(api.build_x0_table);
@@ -586,6 +598,9 @@ PyObject* py_init(PyObject*, PyObject* const* a, Py_ssize_t n) {
     set(api.block_bwd); set(api.takes_pairs); set(api.plane_bytes); set(api.build_plane); set(api.pair_bytes);
     set(api.build_pair); set(api.pair_workspace_bytes); set(api.pair_fwd);
     set(api.takes_planes); set(api.plane_workspace_bytes); set(api.plane_fwd);
+    set(api.residual_norm_fwd); set(api.residual_norm_workspace); set(api.residual_norm_bwd); set(api.clip_workspace);
+    set(api.clip_by_norm); set(api.quantize_tokens); set(api.int8_product); set(api.pointwise_int8_workspace);
+    set(api.pointwise_int8);
     Py_RETURN_NONE;
   });
 }
@@ -604,6 +619,12 @@ PyMethodDef methods[] = {
     {"backward", (PyCFunction)(void (*)(void))py_backward, METH_FASTCALL, nullptr},
     {"block_train", (PyCFunction)(void (*)(void))py_block_train, METH_FASTCALL, nullptr},
     {"block_backward", (PyCFunction)(void (*)(void))py_block_backward, METH_FASTCALL, nullptr},
+    {"residual_norm", (PyCFunction)(void (*)(void))py_residual_norm, METH_FASTCALL, nullptr},
+    {"residual_norm_backward", (PyCFunction)(void (*)(void))py_residual_norm_backward, METH_FASTCALL, nullptr},
+    {"quantize_tokens", (PyCFunction)(void (*)(void))py_quantize_tokens, METH_FASTCALL, nullptr},
+    {"int8_product", (PyCFunction)(void (*)(void))py_int8_product, METH_FASTCALL, nullptr},
+    {"pointwise_int8", (PyCFunction)(void (*)(void))py_pointwise_int8, METH_FASTCALL, nullptr},
+    {"clip_by_norm", (PyCFunction)(void (*)(void))py_clip_by_norm, METH_FASTCALL, nullptr},
     {"block", (PyCFunction)(void (*)(void))py_block, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
@@ -613,7 +634,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, null
 PyMODINIT_FUNC PyInit__host(void) {
   PyObject* m = PyModule_Create(&module);
   if (!m) return nullptr;
-  PyObject* names = Py_BuildValue("(ssssssssssssssssssssssssssssss)", "cvb_strerror", "cvb_last_cuda_error", "cvb_transfer_bytes",
+  PyObject* names = Py_BuildValue("(sssssssssssssssssssssssssssssssssssssss)", "cvb_strerror", "cvb_last_cuda_error", "cvb_transfer_bytes",
                                   "cvb_build_transfer", "cvb_build_x0_table", "cvb_converse2d_workspace_bytes",
                                   "cvb_converse2d_fwd", "cvb_block_pack_bytes", "cvb_block_pack", "cvb_block_pre_fwd",
                                   "cvb_block_post_fwd", "cvb_converse2d_train_workspace_bytes",
@@ -622,7 +643,10 @@ PyMODINIT_FUNC PyInit__host(void) {
                                   "cvb_block_bwd_workspace_bytes", "cvb_block_bwd", "cvb_takes_pairs",
                                   "cvb_plane_transfer_bytes", "cvb_build_plane_transfer", "cvb_pair_transfer_bytes",
                                   "cvb_build_pair_transfer", "cvb_pair_workspace_bytes", "cvb_pair_fwd",
-                                  "cvb_takes_planes", "cvb_plane_workspace_bytes", "cvb_plane_fwd");
+                                  "cvb_takes_planes", "cvb_plane_workspace_bytes", "cvb_plane_fwd",
+                                  "cvb_residual_norm_fwd", "cvb_residual_norm_workspace_bytes", "cvb_residual_norm_bwd",
+                                  "cvb_clip_workspace_bytes", "cvb_clip_by_norm", "cvb_quantize_tokens", "cvb_int8_product",
+                                  "cvb_pointwise_int8_workspace_bytes", "cvb_pointwise_int8");
   if (!names || PyModule_AddObject(m, "names", names) < 0) return nullptr;
   return m;
 }

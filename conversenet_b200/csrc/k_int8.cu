@@ -1,0 +1,496 @@
+// 1x1 products in 8-bit integers: tokens quantised by their largest channel, weights by output channel.
+//
+// Quantisation is decided exactly: q = rint(127 x / a), a the token's largest magnitude.  The product with fp32(127 / a) is off
+// by less than 127 . 2^-23 = 1.6e-5; where it lies nearer than 2e-5 to a half, 254 |x| and (2 m + 1) a are compared, both exact
+// in 64 bits.  So the integers do not depend on the route, the layout or the device.
+//
+// The product: D = L R^T on tcgen05 (kind::i8, sums exact in 32 bits).  The operand whose rows become lanes of tensor memory
+// is the one whose index is contiguous in the output: pixels in channels_first, output channels in channels_last.  So a warp
+// stores 32 neighbours of a row whichever layout it is, straight from its registers.  Both operands are K-major in global
+// memory; TMA brings boxes of 128 bytes of K by 128 (L) or NT (R) rows to shared memory (128-byte swizzle), zeros behind the
+// last K and the last row.  One block a multiprocessor walks over tiles of 128 x NT: a warp that copies, a warp that issues the
+// MMAs, eight warps that scale and store; two accumulators, so that a tile is stored while the next one is computed.
+// Every wait is bounded; a role that gives up sets the status word and ends, and the others follow.
+#include <cuda.h>
+
+#include <atomic>
+
+#include "../../include/converse_b200.h"
+#include "cvb_internal.h"
+#include "cvb_tc.cuh"
+
+namespace cvb {
+namespace i8 {
+
+// ------------------------------------------------------------------ quantisation
+struct QuantParams {
+  const void* x;
+  signed char* q;
+  float* scale;
+  long long B, HW, tokens, ldq;
+  int K, tiles, tpr;
+};
+
+__device__ __forceinline__ float magnitude(float v, float m) {     // the larger magnitude; a NaN counts as the largest
+  return __uint_as_float(max(__float_as_uint(v) & 0x7fffffffu, __float_as_uint(m)));
+}
+struct Quantiser {
+  float up, inv, top;
+  bool bad;
+  __device__ __forceinline__ explicit Quantiser(float a) {
+    bad = __float_as_uint(a) >= 0x7f800000u;
+    up = a < 0x1p-100f ? 0x1p100f : 1.f;           // 127 / a stays finite
+    top = a * up;
+    inv = bad || a == 0.f ? 0.f : __fdiv_rn(127.f, top);
+  }
+  __device__ __forceinline__ float scale(float a) const { return bad ? __uint_as_float(0x7fffffffu) : __fdiv_rn(a, 127.f); }
+  __device__ __forceinline__ int operator()(float x) const {
+    if (bad) return 0;
+    const float t = x * up * inv;
+    float n = rintf(t);
+    if (fabsf(t - n) > 0.49998f) {
+      const float m = floorf(fabsf(t));
+      const double d = 254.0 * (double)fabsf(x * up) - (2.0 * (double)m + 1.0) * (double)top;
+      n = copysignf(d > 0 || (d == 0 && ((int)m & 1)) ? m + 1.f : m, t);
+    }
+    return (int)n;
+  }
+};
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
+  return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 | (uint32_t)d << 24;
+}
+template <typename IO>
+__device__ __forceinline__ float load1(const void* p, long long i);
+template <>
+__device__ __forceinline__ float load1<float>(const void* p, long long i) { return ((const float*)p)[i]; }
+template <>
+__device__ __forceinline__ float load1<__nv_bfloat16>(const void* p, long long i) { return __bfloat162float(((const __nv_bfloat16*)p)[i]); }
+
+// channels_first: 32 pixels a block, warp s takes channels 32 s .. of each group of 32 S; more than one group is read twice
+constexpr int kQuantWarps = 8;
+template <typename IO>
+__global__ void __launch_bounds__(32 * kQuantWarps) quant_first_kernel(const __grid_constant__ QuantParams P) {
+  pdl_start();
+  __shared__ float red[kQuantWarps][32];
+  const int lane = threadIdx.x & 31, s = threadIdx.x >> 5, S = blockDim.x >> 5;
+  const long long b = blockIdx.x / P.tiles, px = (long long)(blockIdx.x - b * P.tiles) * 32 + lane;
+  const bool live = px < P.HW;
+  const long long base = b * P.K * P.HW + (live ? px : P.HW - 1), token = b * P.HW + px;
+  float v[32], a = 0.f;
+  for (int c0 = 32 * s; c0 < P.K; c0 += 32 * S) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = c0 + i < P.K ? load1<IO>(P.x, base + (c0 + i) * P.HW) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) a = magnitude(v[i], a);
+  }
+  if (S > 1) {
+    red[s][lane] = a;
+    __syncthreads();
+    for (int t = 0; t < S; ++t) a = magnitude(red[t][lane], a);
+  }
+  if (!live) return;
+  const Quantiser q(a);
+  if (s == 0) P.scale[token] = q.scale(a);
+  for (int c0 = 32 * s; c0 < P.K; c0 += 32 * S) {
+    if (P.K > 32 * S) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = c0 + i < P.K ? load1<IO>(P.x, base + (c0 + i) * P.HW) : 0.f;
+    }
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = pack4(q(v[4 * i]), q(v[4 * i + 1]), q(v[4 * i + 2]), q(v[4 * i + 3]));
+    signed char* to = P.q + token * P.ldq + c0;
+    *(uint4*)to = make_uint4(w[0], w[1], w[2], w[3]);
+    if (c0 + 16 < P.K) *(uint4*)(to + 16) = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
+// channels_last: `tpr` threads a token, each with vectors of V channels; tokens of more than 16 tpr channels are read twice
+template <typename IO, int V>
+__device__ __forceinline__ void load_vec(const void* p, long long i, float (&v)[V]) {
+  if constexpr (V == 1) {
+    v[0] = load1<IO>(p, i);
+  } else if constexpr (V == 4) {
+    const float4 a = *(const float4*)((const float*)p + i);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  } else {
+    const uint4 a = *(const uint4*)((const __nv_bfloat16*)p + i);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+  }
+}
+template <typename IO, int V>
+__global__ void __launch_bounds__(1024) quant_last_kernel(const __grid_constant__ QuantParams P) {
+  pdl_start();
+  constexpr int NV = 16 / V;
+  __shared__ float red[32];
+  const int tpr = P.tpr, t = threadIdx.x & (tpr - 1), rows = blockDim.x / tpr;
+  const long long token = (long long)blockIdx.x * rows + threadIdx.x / tpr;
+  const bool live = token < P.tokens;
+  const long long base = live ? token * P.K : 0;
+  float v[NV][V], a = 0.f;
+  for (int c0 = 0; c0 < P.K; c0 += 16 * tpr) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = c0 + (i * tpr + t) * V;
+      if (c < P.K) {
+        load_vec<IO, V>(P.x, base + c, v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[i][j] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V; ++j) a = magnitude(v[i][j], a);
+  }
+  for (int o = (tpr < 32 ? tpr : 32) >> 1; o; o >>= 1) a = magnitude(__shfl_xor_sync(0xffffffffu, a, o), a);
+  if (tpr > 32) {
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
+    __syncthreads();
+    const int w0 = (threadIdx.x & ~(tpr - 1)) >> 5;
+    for (int j = 0; j < (tpr >> 5); ++j) a = magnitude(red[w0 + j], a);
+  }
+  if (!live) return;
+  const Quantiser q(a);
+  if (t == 0) P.scale[token] = q.scale(a);
+  for (int c0 = 0; c0 < P.K; c0 += 16 * tpr) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = c0 + (i * tpr + t) * V;
+      if (c >= P.K) continue;
+      if (P.K > 16 * tpr) load_vec<IO, V>(P.x, base + c, v[i]);
+      signed char* to = P.q + token * P.ldq + c;
+      if constexpr (V == 1) {
+        *to = (signed char)q(v[i][0]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; j += 4) *(uint32_t*)(to + j) = pack4(q(v[i][j]), q(v[i][j + 1]), q(v[i][j + 2]), q(v[i][j + 3]));
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ product
+constexpr int kM = 128, kBK = 128;                     // rows of L in a tile; bytes of K in a stage
+constexpr int kEpilogueWarps = 8, kThreads = 32 * (4 + kEpilogueWarps);
+constexpr int kPolls = 1 << 20;
+
+struct ProductParams {
+  const float *l_scale, *r_scale, *l_bias, *r_bias;    // by row of L (of all images), by row of R
+  void* out;
+  long long images, rows, cols;        // of each image: rows of L, and of R
+  long long image_stride, ldc;         // elements of the output
+  int K, row_tiles, col_tiles;
+  long long tiles;
+  int* status;
+};
+
+__host__ __device__ constexpr int stages_of(int NT) { return NT == 256 ? 4 : NT == 128 ? 6 : 8; }
+__host__ __device__ constexpr int stage_bytes(int NT) { return (kM + NT) * kBK; }
+
+__device__ __forceinline__ uint64_t swizzled_desc(const void* p) {
+  uint64_t d = (uint64_t)((smem_u32(p) >> 4) & 0x3FFF);
+  d |= (uint64_t)1 << 16;                              // (not read for swizzled K-major operands)
+  d |= (uint64_t)(1024 >> 4) << 32;                    // eight rows of 128 bytes
+  d |= (uint64_t)1 << 46;                              // version
+  d |= (uint64_t)2 << 61;                              // 128-byte swizzle
+  return d;
+}
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add, uint32_t elected) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
+      "}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u), "r"(elected)
+      : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar, uint32_t elected) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred e;\n\t"
+      "setp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t"
+      "}\n" ::"r"(smem_u32(bar)), "r"(elected)
+      : "memory");
+}
+__device__ __forceinline__ void tma_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld32i(uint32_t taddr, int (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// every lane waits, and all of them learn the same
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, kPolls));
+}
+
+struct Tile {
+  long long image;
+  int row, col;          // first row of L in the image, first row of R
+  __device__ __forceinline__ Tile(const ProductParams& P, long long t, int NT) {
+    const long long r = t / P.col_tiles;
+    col = (int)(t - r * P.col_tiles) * NT;
+    image = r / P.row_tiles;
+    row = (int)(r - image * P.row_tiles) * kM;
+  }
+};
+
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+template <typename IO, int NT>
+__global__ void __launch_bounds__(kThreads, 1)
+product_kernel(const __grid_constant__ CUtensorMap mapL, const __grid_constant__ CUtensorMap mapR,
+               const __grid_constant__ ProductParams P) {
+  constexpr int ST = stages_of(NT);
+  extern __shared__ unsigned char dynamic[];
+  unsigned char* const ring = dynamic + (-smem_u32(dynamic) & 1023);       // the swizzle counts from 1024-byte boundaries
+  __shared__ uint64_t full[ST], empty[ST], done[2], free_[2], drained;
+  __shared__ uint32_t tmem_base;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // Before tensor memory is taken: a block of the kernel before, waiting for it, would wait for this one.
+  pdl_start();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < ST; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&done[i], 1), mbar_init(&free_[i], kEpilogueWarps);
+    mbar_init(&drained, 1);
+    mbar_fence_init();
+  }
+  if (warp == 2) tc::tmem_alloc(&tmem_base, 2 * NT);
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_base;
+  const int kblocks = (P.K + kBK - 1) / kBK;
+  bool ok = true;
+  if (warp == 0) {
+    // copies
+    if (lane == 0) {
+      int st = 0;
+      uint32_t ph = 0;
+      long long issued = 0;
+      for (long long t = blockIdx.x; t < P.tiles && ok; t += gridDim.x) {
+        const Tile tile(P, t, NT);
+        const int row = (int)(tile.image * P.rows) + tile.row;
+        for (int k = 0; k < kblocks; ++k) {
+          ok = mbar_wait_bounded(&empty[st], ph ^ 1, kPolls);
+          if (!ok) break;
+          unsigned char* at = ring + st * stage_bytes(NT);
+          mbar_expect_tx(&full[st], stage_bytes(NT));
+          tma_2d(at, &mapL, k * kBK, row, &full[st]);
+          tma_2d(at + kM * kBK, &mapR, k * kBK, tile.col, &full[st]);
+          ++issued;
+          if (++st == ST) st = 0, ph ^= 1;
+        }
+      }
+      if (!ok) {
+        // no copy may be in flight when the block ends
+        for (int i = 0; i < ST; ++i) {
+          const long long uses = issued > i ? (issued - 1 - i) / ST + 1 : 0;
+          if (uses) mbar_wait_bounded(&full[i], (uint32_t)((uses - 1) & 1), kPolls);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // MMAs
+    const uint32_t elected = tc::elect_one();
+    const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(NT >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
+    int st = 0, acc = 0;
+    uint32_t ph = 0, aph = 0;
+    for (long long t = blockIdx.x; t < P.tiles && ok; t += gridDim.x) {
+      ok = warp_wait(&free_[acc], aph ^ 1);
+      if (!ok) break;
+      tc::fence_after_sync();
+      for (int k = 0; k < kblocks; ++k) {
+        ok = warp_wait(&full[st], ph);
+        if (!ok) break;
+        tc::fence_after_sync();
+        const unsigned char* at = ring + st * stage_bytes(NT);
+        const uint64_t a = swizzled_desc(at), b = swizzled_desc(at + kM * kBK);
+        const int steps = min(kBK / 32, (P.K - k * kBK + 31) / 32);
+        for (int s = 0; s < steps; ++s) mma_i8(tmem + acc * NT, a + 2 * s, b + 2 * s, idesc, (k | s) != 0, elected);
+        commit(&empty[st], elected);
+        if (++st == ST) st = 0, ph ^= 1;
+      }
+      if (!ok) break;
+      commit(&done[acc], elected);
+      if (acc) aph ^= 1;
+      acc ^= 1;
+    }
+    commit(&drained, elected);
+    if (!warp_wait(&drained, 0)) ok = false;
+  } else if (warp >= 4) {
+    // lane r of quadrant w & 3; the two warps of a quadrant take half of the columns each
+    const int quadrant = warp & 3, half = (warp - 4) >> 2;
+    int acc = 0;
+    uint32_t aph = 0;
+    for (long long t = blockIdx.x; t < P.tiles; t += gridDim.x) {
+      const Tile tile(P, t, NT);
+      const long long r = tile.row + quadrant * 32 + lane;
+      const bool live = r < P.rows;
+      const float ls = live ? P.l_scale[tile.image * P.rows + r] : 0.f, lb = live && P.l_bias ? P.l_bias[r] : 0.f;
+      IO* out = (IO*)P.out + tile.image * P.image_stride + r;
+      ok = warp_wait(&done[acc], aph);
+      if (!ok) break;
+      tc::fence_after_sync();
+      for (int c0 = half * (NT / 2); c0 < (half + 1) * (NT / 2); c0 += 32) {
+        const long long c = tile.col + c0;
+        if (c >= P.cols) break;
+        const float rs = c + lane < P.cols ? P.r_scale[c + lane] : 0.f;
+        const float rb = c + lane < P.cols && P.r_bias ? P.r_bias[c + lane] : 0.f;
+        int v[32];
+        tmem_ld32i(tmem + acc * NT + c0 + ((uint32_t)(quadrant * 32) << 16), v);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const float s = __shfl_sync(0xffffffffu, rs, j), o = __shfl_sync(0xffffffffu, rb, j);
+          if (live && c + j < P.cols) store1(out + (c + j) * P.ldc, fmaf((float)v[j] * ls, s, o + lb));
+        }
+      }
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&free_[acc]);
+      if (acc) aph ^= 1;
+      acc ^= 1;
+    }
+  }
+  if (!ok && lane == 0 && P.status) *P.status = 1;
+  __syncwarp();
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  if (warp == 2) tc::tmem_dealloc(tmem, 2 * NT);
+}
+
+// ------------------------------------------------------------------ launches
+static int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static int encode_tiled(EncodeTiled* out) {
+  static std::atomic<EncodeTiled> known{nullptr};          // (looked up twice at worst)
+  EncodeTiled fn = known.load(std::memory_order_acquire);
+  if (!fn) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    CVB_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found));
+    if (found != cudaDriverEntryPointSuccess || !p) return CVB_ERR_CUDA;
+    fn = (EncodeTiled)p;
+    known.store(fn, std::memory_order_release);
+  }
+  *out = fn;
+  return CVB_OK;
+}
+// rows x K bytes, boxes of 128 bytes x box_rows
+static int row_map(CUtensorMap* m, const signed char* p, long long rows, int K, long long ld, int box_rows) {
+  EncodeTiled encode;
+  const int rc = encode_tiled(&encode);
+  if (rc != CVB_OK) return rc;
+  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {kBK, (cuuint32_t)box_rows}, step[2] = {1, 1};
+  return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)p, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? CVB_OK : CVB_ERR_BAD_ARGUMENT;
+}
+
+template <typename IO>
+static int quantize(QuantParams& P, bool last, cudaStream_t st) {
+  if (!last) {
+    P.tiles = ceil_div(P.HW, 32);
+    const int S = min(kQuantWarps, ceil_div(P.K, 32));
+    return launch_chained(quant_first_kernel<IO>, dim3((unsigned)(P.tiles * P.B)), 32 * S, 0, st, P);
+  }
+  constexpr int V = 16 / (int)sizeof(IO);
+  P.tpr = 4;
+  while (P.tpr < 1024 && 16 * P.tpr < P.K) P.tpr *= 2;
+  const int threads = P.tpr > 256 ? P.tpr : 256;
+  const dim3 grid((unsigned)ceil_div(P.tokens, threads / P.tpr));
+  if (P.K % V == 0 && (size_t)P.x % 16 == 0) return launch_chained(quant_last_kernel<IO, V>, grid, threads, 0, st, P);
+  return launch_chained(quant_last_kernel<IO, 1>, grid, threads, 0, st, P);
+}
+
+template <typename IO, int NT>
+static int product(ProductParams& P, const signed char* l, long long lrows, long long ldl, const signed char* r, long long rrows,
+                   long long ldr, int sms, cudaStream_t st) {
+  CUtensorMap mapL, mapR;
+  int rc = row_map(&mapL, l, lrows, P.K, ldl, kM);
+  if (rc == CVB_OK) rc = row_map(&mapR, r, rrows, P.K, ldr, NT);
+  if (rc != CVB_OK) return rc;
+  P.row_tiles = ceil_div(P.rows, kM);
+  P.col_tiles = ceil_div(P.cols, NT);
+  P.tiles = P.images * P.row_tiles * P.col_tiles;
+  const size_t smem = (size_t)stages_of(NT) * stage_bytes(NT) + 1024;
+  CVB_CUDA(cudaFuncSetAttribute(product_kernel<IO, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  return launch_chained(product_kernel<IO, NT>, dim3((unsigned)(P.tiles < sms ? P.tiles : sms)), kThreads, smem, st, mapL, mapR, P);
+}
+template <typename IO>
+static int product_any(const signed char* q, long long ldq, const float* scale, const signed char* w, long long ldw,
+                       const float* w_scale, const float* bias, void* out, long long B, long long HW, int K, int N, bool last,
+                       int sms, int* status, cudaStream_t st) {
+  ProductParams P;
+  memset(&P, 0, sizeof(P));
+  P.out = out; P.K = K; P.status = status;
+  const long long tokens = B * HW;
+  if (last) {
+    P.l_scale = w_scale; P.l_bias = bias; P.r_scale = scale;
+    P.images = 1; P.rows = N; P.cols = tokens; P.ldc = N;
+  } else {
+    P.l_scale = scale; P.r_scale = w_scale; P.r_bias = bias;
+    P.images = B; P.rows = HW; P.cols = N; P.ldc = HW; P.image_stride = (long long)N * HW;
+  }
+  const signed char *l = last ? w : q, *r = last ? q : w;
+  const long long lrows = last ? N : tokens, rrows = last ? tokens : N, ldl = last ? ldw : ldq, ldr = last ? ldq : ldw;
+  // the widest tile that leaves a tile for every multiprocessor
+  auto tiles = [&](int NT) { return P.images * ceil_div(P.rows, kM) * ceil_div(P.cols, NT); };
+  if (P.cols > 128 && tiles(256) >= sms) return product<IO, 256>(P, l, lrows, ldl, r, rrows, ldr, sms, st);
+  if (P.cols > 64 && tiles(128) >= sms) return product<IO, 128>(P, l, lrows, ldl, r, rrows, ldr, sms, st);
+  return product<IO, 64>(P, l, lrows, ldl, r, rrows, ldr, sms, st);
+}
+
+int run_quantize(const void* x, signed char* q, float* scale, long long B, long long HW, int K, long long ldq, bool last, int io,
+                 cudaStream_t st) {
+  QuantParams P;
+  P.x = x; P.q = q; P.scale = scale; P.B = B; P.HW = HW; P.tokens = B * HW; P.ldq = ldq; P.K = K; P.tiles = P.tpr = 0;
+  return io == CVB_F32 ? quantize<float>(P, last, st) : quantize<__nv_bfloat16>(P, last, st);
+}
+int run_product(const signed char* q, long long ldq, const float* scale, const signed char* w, long long ldw, const float* w_scale,
+                const float* bias, void* out, long long B, long long HW, int K, int N, bool last, int io, int sms, int* status,
+                cudaStream_t st) {
+  return io == CVB_F32 ? product_any<float>(q, ldq, scale, w, ldw, w_scale, bias, out, B, HW, K, N, last, sms, status, st)
+                       : product_any<__nv_bfloat16>(q, ldq, scale, w, ldw, w_scale, bias, out, B, HW, K, N, last, sms, status, st);
+}
+size_t workspace(long long B, long long HW, int K, int N, bool last, int io) {
+  const long long tokens = B * HW;
+  (void)N; (void)last; (void)io;
+  return ((size_t)tokens * ((K + 15) / 16 * 16) + 255) / 256 * 256 + (size_t)tokens * sizeof(float);
+}
+int run_pointwise(const void* x, const signed char* w, long long ldw, const float* w_scale, const float* bias, void* out,
+                  long long B, long long HW, int K, int N, bool last, int io, void* ws, int sms, int* status, cudaStream_t st) {
+  const long long ldq = (K + 15) / 16 * 16, tokens = B * HW;
+  signed char* q = (signed char*)ws;
+  float* scale = (float*)((char*)ws + ((size_t)tokens * ldq + 255) / 256 * 256);
+  const int rc = run_quantize(x, q, scale, B, HW, K, ldq, last, io, st);
+  return rc != CVB_OK ? rc : run_product(q, ldq, scale, w, ldw, w_scale, bias, out, B, HW, K, N, last, io, sms, status, st);
+}
+
+}  // namespace i8
+}  // namespace cvb

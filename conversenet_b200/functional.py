@@ -207,3 +207,120 @@ def pw_res(t, res, conv, alpha=None):
                                 _stream_ptr(res.device))
     _cabi.check(rc, "cvb_pw_res_fwd")
     return out
+
+
+DATA_FORMATS = ("channels_first", "channels_last")
+
+
+def _channels_last(data_format):
+    if data_format not in DATA_FORMATS:
+        raise ValueError("data_format must be 'channels_first' | 'channels_last', got: %r" % (data_format,))
+    return data_format == "channels_last"
+
+
+def residual_norm(x, branch, scale=None, gate=None, post_weight=None, post_bias=None, pre_weight=None, pre_bias=None, eps=1e-5,
+                  norm="layer", gate_act=None, data_format="channels_first"):
+    """The seam between two branches of a block, of any width, as one kernel:
+
+        y = x + scale * act(gate) * N_post(branch),    z = N_pre(y)
+
+    where the norms run over the channels: `norm` "layer" (mean and biased variance, as `LayerNorm`) or "rms" (root of the
+    mean square), with `post_weight` / `pre_weight` and optional biases.  Without `post_weight` the branch is taken as it is;
+    without `pre_weight` the result is y, else (y, z).  `scale` holds a value for each channel (the alphas of
+    `ConverseBlockAlphaVariant`), `gate` one for each element or for each image and channel ((B,C,1,1), or (B,1,...,C) in
+    channels_last); `gate_act` is None or "sigmoid".  x and branch: (B,C,H,W), or (...,C) in channels_last, float32 or
+    bfloat16, both of one type; strided tensors are copied.  z comes from y before it is rounded to that type.
+
+    Differentiable in every tensor (once).  Up to 16384 channels, with gradients in channels_first 4096."""
+    last = _channels_last(data_format)
+    if norm not in ("layer", "rms"):
+        raise ValueError("norm must be 'layer' | 'rms', got: %r" % (norm,))
+    if gate_act not in (None, "sigmoid"):
+        raise ValueError("gate_act must be None | 'sigmoid', got: %r" % (gate_act,))
+    args = (branch, scale, gate, post_weight, post_bias, pre_weight, pre_bias)
+    cfg = (float(eps), norm == "rms", gate_act is not None, last)
+    if torch.is_grad_enabled() and (x.requires_grad or any(t is not None and t.requires_grad for t in args)):
+        from .autograd import ResidualNormFunction
+        y, z = ResidualNormFunction.apply(cfg, x, *args)
+    else:
+        y, z, _ = _cabi.host().residual_norm(x, *args, *cfg, False)
+    return y if pre_weight is None else (y, z)
+
+
+_NORM_KINDS = {1.0: 1, 2.0: 2, float("inf"): 0}
+
+
+def _norm_kind(norm_type):
+    kind = _NORM_KINDS.get(float(norm_type))
+    if kind is None:
+        raise ValueError("norm_type must be 1, 2 or inf, got: %r" % (norm_type,))
+    return kind
+
+
+def grad_norm(tensors, norm_type=2.0):
+    """The norm of all tensors together, a float32 tensor on their device (sums in 64 bits; the same bits at every call)."""
+    return _clip_norm(tensors, False, norm_type, 0.0)[1]
+
+
+def clip_by_global_norm(tensors, max_norm, norm_type=2.0, out=None):
+    """(the tensors times min(1, max_norm / (norm + 1e-6)), norm): `grad_norm`'s norm, and the tensors scaled so that it does
+    not exceed `max_norm`.  `out`: tensors of the same shapes, float32 or bfloat16 whatever the inputs are (master gradients
+    in 32 bits), that receive them; they may be the tensors themselves.  Not differentiable."""
+    return _clip_norm(tensors, out, norm_type, max_norm)
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """`torch.nn.utils.clip_grad_norm_` in two kernels for all gradients: scales the parameters' gradients in place and
+    returns their norm.  Gradients whose norm is small enough are not written.  `error_if_nonfinite` waits for the norm."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if error_if_nonfinite and not bool(torch.isfinite(grad_norm(grads, norm_type))):
+        raise RuntimeError("The total norm of order %s for gradients is not finite, so they cannot be clipped" % norm_type)
+    return _clip_norm(grads, True, norm_type, max_norm)[1]
+
+
+def _clip_norm(tensors, out, norm_type, max_norm):
+    kind = _norm_kind(norm_type)
+    tensors = tensors if isinstance(tensors, (list, tuple)) else list(tensors)
+    if not tensors:
+        return [], torch.tensor(0.0)
+    return _cabi.host().clip_by_norm(tensors, out, kind, float(max_norm))
+
+
+def _forward_only(what, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("%s is for inference: call it under torch.no_grad()" % what)
+
+
+def quantize_tokens(x, data_format="channels_first"):
+    """8-bit integers and a scale for every token: scale = max |x| / 127 over its channels, q = the integer nearest to x /
+    scale (an even one where two are as near), decided exactly.  x (B,C,H,W) or, channels_last, (...,C), float32 or bfloat16;
+    q (B,H,W,C) or (...,C) int8 with rows at multiples of 16 bytes, scale without the last dimension, float32.  A token with
+    an infinity or a NaN gets the scale NaN."""
+    _forward_only("quantize_tokens", x)
+    return _cabi.host().quantize_tokens(x, _channels_last(data_format))
+
+
+def quantize_weight(weight):
+    """A 1x1 convolution's or linear layer's weight (N,K[,1,1]) as 8-bit integers (N,K) and a scale for each output channel:
+    `quantize_tokens` of its rows, rows at multiples of 16 bytes as `pointwise_int8` reads them without a copy."""
+    return _cabi.host().quantize_tokens(weight.detach().flatten(1), True)
+
+
+def int8_product(q, scale, weight_q, weight_scale, bias=None, dtype=torch.float32, data_format="channels_last"):
+    """out[t, n] = (sum_k q[t, k] weight_q[n, k]) scale[t] weight_scale[n] + bias[n] on the tensor cores, the sum exact in 32
+    bits (K up to 131072).  q (...,K) int8, scale for each of its rows, weight_q (N,K) int8.  The result, float32 or bfloat16,
+    is (...,N), or (B,N,H,W) in channels_first, which takes q as (B,H,W,K).  Rows of q and weight_q that do not begin at
+    multiples of 16 bytes are copied."""
+    _forward_only("int8_product", scale, weight_scale, bias)
+    if dtype not in (torch.float32, torch.bfloat16):
+        raise RuntimeError("int8_product gives float32 or bfloat16 tensors, not %s" % dtype)
+    return _cabi.host().int8_product(q, scale, weight_q, weight_scale, bias, dtype == torch.bfloat16, _channels_last(data_format))
+
+
+def pointwise_int8(x, weight_q, weight_scale, bias=None, data_format="channels_first"):
+    """A 1x1 convolution (or, channels_last, a linear layer) in 8-bit integers: `quantize_tokens` of x, then `int8_product`
+    in the type of x.  `weight_q`, `weight_scale`: from `quantize_weight`."""
+    _forward_only("pointwise_int8", x, weight_scale, bias)
+    return _cabi.host().pointwise_int8(x, weight_q, weight_scale, bias, _channels_last(data_format))

@@ -337,6 +337,79 @@ int cvb_tap_gradient(const float* g_full, const float* r, float* out, int nseg, 
                      int s, void* stream);
 
 /*
+ * The seam between two branches of a block of any width C: the branch's output normalised, gated, scaled and added to the
+ * residual, and the sum normalised for the next branch, as one kernel:
+ *     y = x + scale . s(gate) . N_post(branch),   z = N_pre(y)
+ * N: LayerNorm, or RMS norm (`rms`), over the channels of a token with weights (and biases); without post_w the branch is
+ * taken as it is, without pre_w there is no z.  s: the identity or the sigmoid (`gate_act` 1).  (The reference runs LayerNorm,
+ * the branch scale and the residual as separate tensors, models/util_converse.py:60-68,321-322.)
+ *   tensors  : channels_last 0: (B,C,HW); 1: (B,HW,C); contiguous, io_dtype
+ *   gate     : CVB_GATE_FULL like branch; CVB_GATE_IMAGE (B,C) fp32
+ *   stats    : 4 B HW floats kept for the gradients, or NULL
+ * Backward, from dy = dL/dy and dz = dL/dz (either may be NULL), reading x (where dz is given), branch, gate and stats:
+ * dx, dbranch, dgate (of the gate's layout and type) and the gradients of the vectors (each may be NULL).
+ * C: up to 16384; backward in channels_first up to 4096 (CVB_ERR_TOO_LARGE).  The workspace is needed by the backward only.
+ */
+enum { CVB_GATE_NONE = 0, CVB_GATE_FULL = 1, CVB_GATE_IMAGE = 2 };
+typedef struct {
+  const void *x, *branch, *gate;
+  void *y, *z;
+  const float *scale, *post_w, *post_b, *pre_w, *pre_b;
+  float* stats;
+  const void *dy, *dz;
+  void *dx, *dbranch, *dgate;
+  float *dscale, *dpost_w, *dpost_b, *dpre_w, *dpre_b;
+  long long B, HW;
+  int C, channels_last, rms, gate_kind, gate_act, io_dtype;
+  float eps;
+  void* workspace;
+  size_t workspace_bytes;
+  void* stream;
+} cvb_residual_norm_args;
+int cvb_residual_norm_fwd(const cvb_residual_norm_args* args);
+size_t cvb_residual_norm_workspace_bytes(int C, long long B, int gate_kind);
+int cvb_residual_norm_bwd(const cvb_residual_norm_args* args);
+
+/*
+ * The norm of `count` tensors together (kind 1: sum of magnitudes, 2: Euclidean, 0: largest magnitude) and, with `scale_them`,
+ * out = in . min(1, max_norm / (norm + 1e-6)) for each: what training does with its gradients before a step.
+ *   spans : host array; in, out device pointers aligned to their elements; out may be in (same type) and overlaps nothing else
+ *   norm  : device float
+ * Sums in 64 bits, in an order of their own: equal calls give equal bits.  Infinities and NaN reach the norm; out is then what
+ * the formula gives.  Where in is out and the norm is small enough, nothing is written to it.
+ */
+typedef struct {
+  const void* in;
+  void* out;
+  long long n;              /* elements, 0 to 2^45 */
+  int in_type, out_type;    /* CVB_F32, CVB_BF16 */
+} cvb_span;
+size_t cvb_clip_workspace_bytes(int count);
+int cvb_clip_by_norm(const cvb_span* spans, int count, int kind, double max_norm, int scale_them, float* norm,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * 1x1 products in 8-bit integers.  A token t of K channels becomes integers and a scale,
+ *     scale_t = max_k |x_tk| / 127,   q_tk = the integer nearest to x_tk / scale_t (an even one where two are as near),
+ * decided exactly; weights are integers with a scale for each output channel, and
+ *     out_tn = (sum_k q_tk w_nk) . scale_t . w_scale_n + bias_n,
+ * the sum exact in 32-bit integers (K up to 131072).  A token with an infinity or a NaN gets the scale NaN, and so NaN outputs.
+ *   cvb_quantize_tokens : x channels_last 0: (B,K,HW); 1: (B,HW,K), contiguous, io_dtype -> q (B HW rows of ldq bytes), scale
+ *   cvb_int8_product    : q (B HW rows), w (N rows): rows of ldq and ldw bytes, multiples of 16, both addresses 16-byte aligned;
+ *                         out channels_last 0: (B,N,HW); 1: (B,HW,N); bias (N) or NULL
+ *   cvb_pointwise_int8  : the two together; the workspace holds q and the scales where they are not made on the way
+ */
+int cvb_quantize_tokens(const void* x, signed char* q, float* scale, long long B, long long HW, int K, long long ldq,
+                        int channels_last, int io_dtype, void* stream);
+int cvb_int8_product(const signed char* q, long long ldq, const float* scale, const signed char* w, long long ldw,
+                     const float* w_scale, const float* bias, void* out, long long B, long long HW, int K, int N,
+                     int channels_last, int io_dtype, void* stream);
+size_t cvb_pointwise_int8_workspace_bytes(long long B, long long HW, int K, int N, int channels_last, int io_dtype);
+int cvb_pointwise_int8(const void* x, const signed char* w, long long ldw, const float* w_scale, const float* bias, void* out,
+                       long long B, long long HW, int K, int N, int channels_last, int io_dtype, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/*
  * Describe the FFT plan chosen for a padded length n: writes up to max_stages
  * radices, returns the stage count, 0 if n is unsupported.  Host-only, no GPU.
  */
