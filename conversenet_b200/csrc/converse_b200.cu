@@ -817,7 +817,7 @@ int cvb_int8_product(const signed char* q, long long ldq, const float* scale, co
 
 size_t cvb_pointwise_int8_workspace_bytes(long long B, long long HW, int K, int N, int channels_last, int io_dtype) {
   if (check_int8(B, HW, K, io_dtype) != CVB_OK || N < 1) return 0;
-  return i8::workspace(B, HW, K, N, channels_last != 0, io_dtype);
+  return i8::workspace(B, HW, K, N, channels_last != 0, io_dtype, sm_count());
 }
 
 int cvb_pointwise_int8(const void* x, const signed char* w, long long ldw, const float* w_scale, const float* bias, void* out,
@@ -826,7 +826,7 @@ int cvb_pointwise_int8(const void* x, const signed char* w, long long ldw, const
   const int rc = check_int8(B, HW, K, io_dtype);
   if (rc != CVB_OK) return rc;
   if (!x || !int8_rows(w, ldw, K) || !w_scale || !out || N < 1) return CVB_ERR_BAD_ARGUMENT;
-  const size_t need = i8::workspace(B, HW, K, N, channels_last != 0, io_dtype);
+  const size_t need = i8::workspace(B, HW, K, N, channels_last != 0, io_dtype, sm_count());
   if (need && (!workspace || (size_t)workspace % 16 || workspace_bytes < need)) return CVB_ERR_WORKSPACE;
   return i8::run_pointwise(x, w, ldw, w_scale, bias, out, B, HW, K, N, channels_last != 0, io_dtype, workspace, sm_count(),
                            status_ptr(), (cudaStream_t)stream);

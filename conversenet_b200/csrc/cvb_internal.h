@@ -127,7 +127,11 @@ int run_quantize(const void* x, signed char* q, float* scale, long long B, long 
 int run_product(const signed char* q, long long ldq, const float* scale, const signed char* w, long long ldw, const float* w_scale,
                 const float* bias, void* out, long long B, long long HW, int K, int N, bool last, int io, int sms, int* status,
                 cudaStream_t st);
-size_t workspace(long long B, long long HW, int K, int N, bool last, int io);
+// channels_first, quantised on the way to the product (k_int8_planes.cu), for the sizes that planes_take answers true for
+bool planes_take(long long B, long long HW, int K, int N, int io, int sms);
+int run_planes(const void* x, const signed char* w, long long ldw, const float* w_scale, const float* bias, void* out, long long B,
+               long long HW, int K, int N, int io, int sms, int* status, cudaStream_t st);
+size_t workspace(long long B, long long HW, int K, int N, bool last, int io, int sms);
 int run_pointwise(const void* x, const signed char* w, long long ldw, const float* w_scale, const float* bias, void* out,
                   long long B, long long HW, int K, int N, bool last, int io, void* ws, int sms, int* status, cudaStream_t st);
 }  // namespace i8

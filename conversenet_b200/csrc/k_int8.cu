@@ -1,9 +1,5 @@
 // 1x1 products in 8-bit integers: tokens quantised by their largest channel, weights by output channel.
 //
-// Quantisation is decided exactly: q = rint(127 x / a), a the token's largest magnitude.  The product with fp32(127 / a) is off
-// by less than 127 . 2^-23 = 1.6e-5; where it lies nearer than 2e-5 to a half, 254 |x| and (2 m + 1) a are compared, both exact
-// in 64 bits.  So the integers do not depend on the route, the layout or the device.
-//
 // The product: D = L R^T on tcgen05 (kind::i8, sums exact in 32 bits).  The operand whose rows become lanes of tensor memory
 // is the one whose index is contiguous in the output: pixels in channels_first, output channels in channels_last.  So a warp
 // stores 32 neighbours of a row whichever layout it is, straight from its registers.  Both operands are K-major in global
@@ -16,6 +12,7 @@
 #include <atomic>
 
 #include "../../include/converse_b200.h"
+#include "cvb_int8.cuh"
 #include "cvb_internal.h"
 #include "cvb_tc.cuh"
 
@@ -31,34 +28,6 @@ struct QuantParams {
   int K, tiles, tpr;
 };
 
-__device__ __forceinline__ float magnitude(float v, float m) {     // the larger magnitude; a NaN counts as the largest
-  return __uint_as_float(max(__float_as_uint(v) & 0x7fffffffu, __float_as_uint(m)));
-}
-struct Quantiser {
-  float up, inv, top;
-  bool bad;
-  __device__ __forceinline__ explicit Quantiser(float a) {
-    bad = __float_as_uint(a) >= 0x7f800000u;
-    up = a < 0x1p-100f ? 0x1p100f : 1.f;           // 127 / a stays finite
-    top = a * up;
-    inv = bad || a == 0.f ? 0.f : __fdiv_rn(127.f, top);
-  }
-  __device__ __forceinline__ float scale(float a) const { return bad ? __uint_as_float(0x7fffffffu) : __fdiv_rn(a, 127.f); }
-  __device__ __forceinline__ int operator()(float x) const {
-    if (bad) return 0;
-    const float t = x * up * inv;
-    float n = rintf(t);
-    if (fabsf(t - n) > 0.49998f) {
-      const float m = floorf(fabsf(t));
-      const double d = 254.0 * (double)fabsf(x * up) - (2.0 * (double)m + 1.0) * (double)top;
-      n = copysignf(d > 0 || (d == 0 && ((int)m & 1)) ? m + 1.f : m, t);
-    }
-    return (int)n;
-  }
-};
-__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
-  return (uint32_t)(a & 255) | (uint32_t)(b & 255) << 8 | (uint32_t)(c & 255) << 16 | (uint32_t)d << 24;
-}
 template <typename IO>
 __device__ __forceinline__ float load1(const void* p, long long i);
 template <>
@@ -81,16 +50,16 @@ __global__ void __launch_bounds__(32 * kQuantWarps) quant_first_kernel(const __g
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = c0 + i < P.K ? load1<IO>(P.x, base + (c0 + i) * P.HW) : 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) a = magnitude(v[i], a);
+    for (int i = 0; i < 32; i += 2) a = largest(a, v[i], v[i + 1]);
   }
   if (S > 1) {
     red[s][lane] = a;
     __syncthreads();
-    for (int t = 0; t < S; ++t) a = magnitude(red[t][lane], a);
+    for (int t = 0; t < S; ++t) a = largest(a, red[t][lane]);
   }
   if (!live) return;
   const Quantiser q(a);
-  if (s == 0) P.scale[token] = q.scale(a);
+  if (s == 0) P.scale[token] = q.scale();
   for (int c0 = 32 * s; c0 < P.K; c0 += 32 * S) {
     if (P.K > 32 * S) {
 #pragma unroll
@@ -98,7 +67,7 @@ __global__ void __launch_bounds__(32 * kQuantWarps) quant_first_kernel(const __g
     }
     uint32_t w[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = pack4(q(v[4 * i]), q(v[4 * i + 1]), q(v[4 * i + 2]), q(v[4 * i + 3]));
+    for (int i = 0; i < 8; ++i) w[i] = q.four(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
     signed char* to = P.q + token * P.ldq + c0;
     *(uint4*)to = make_uint4(w[0], w[1], w[2], w[3]);
     if (c0 + 16 < P.K) *(uint4*)(to + 16) = make_uint4(w[4], w[5], w[6], w[7]);
@@ -144,18 +113,18 @@ __global__ void __launch_bounds__(1024) quant_last_kernel(const __grid_constant_
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int j = 0; j < V; ++j) a = magnitude(v[i][j], a);
+      for (int j = 0; j < V; ++j) a = largest(a, v[i][j]);
   }
-  for (int o = (tpr < 32 ? tpr : 32) >> 1; o; o >>= 1) a = magnitude(__shfl_xor_sync(0xffffffffu, a, o), a);
+  for (int o = (tpr < 32 ? tpr : 32) >> 1; o; o >>= 1) a = largest(a, __shfl_xor_sync(0xffffffffu, a, o));
   if (tpr > 32) {
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
     __syncthreads();
     const int w0 = (threadIdx.x & ~(tpr - 1)) >> 5;
-    for (int j = 0; j < (tpr >> 5); ++j) a = magnitude(red[w0 + j], a);
+    for (int j = 0; j < (tpr >> 5); ++j) a = largest(a, red[w0 + j]);
   }
   if (!live) return;
   const Quantiser q(a);
-  if (t == 0) P.scale[token] = q.scale(a);
+  if (t == 0) P.scale[token] = q.scale();
   for (int c0 = 0; c0 < P.K; c0 += 16 * tpr) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -164,10 +133,10 @@ __global__ void __launch_bounds__(1024) quant_last_kernel(const __grid_constant_
       if (P.K > 16 * tpr) load_vec<IO, V>(P.x, base + c, v[i]);
       signed char* to = P.q + token * P.ldq + c;
       if constexpr (V == 1) {
-        *to = (signed char)q(v[i][0]);
+        *to = (signed char)q.four(v[i][0], 0.f, 0.f, 0.f);
       } else {
 #pragma unroll
-        for (int j = 0; j < V; j += 4) *(uint32_t*)(to + j) = pack4(q(v[i][j]), q(v[i][j + 1]), q(v[i][j + 2]), q(v[i][j + 3]));
+        for (int j = 0; j < V; j += 4) *(uint32_t*)(to + j) = q.four(v[i][j], v[i][j + 1], v[i][j + 2], v[i][j + 3]);
       }
     }
   }
@@ -478,13 +447,16 @@ int run_product(const signed char* q, long long ldq, const float* scale, const s
   return io == CVB_F32 ? product_any<float>(q, ldq, scale, w, ldw, w_scale, bias, out, B, HW, K, N, last, sms, status, st)
                        : product_any<__nv_bfloat16>(q, ldq, scale, w, ldw, w_scale, bias, out, B, HW, K, N, last, sms, status, st);
 }
-size_t workspace(long long B, long long HW, int K, int N, bool last, int io) {
+// where x is quantised on the way there is no workspace
+size_t workspace(long long B, long long HW, int K, int N, bool last, int io, int sms) {
   const long long tokens = B * HW;
-  (void)N; (void)last; (void)io;
+  if (!last && planes_take(B, HW, K, N, io, sms)) return 0;
   return ((size_t)tokens * ((K + 15) / 16 * 16) + 255) / 256 * 256 + (size_t)tokens * sizeof(float);
 }
 int run_pointwise(const void* x, const signed char* w, long long ldw, const float* w_scale, const float* bias, void* out,
                   long long B, long long HW, int K, int N, bool last, int io, void* ws, int sms, int* status, cudaStream_t st) {
+  if (!last && planes_take(B, HW, K, N, io, sms))
+    return run_planes(x, w, ldw, w_scale, bias, out, B, HW, K, N, io, sms, status, st);
   const long long ldq = (K + 15) / 16 * 16, tokens = B * HW;
   signed char* q = (signed char*)ws;
   float* scale = (float*)((char*)ws + ((size_t)tokens * ldq + 255) / 256 * 256);

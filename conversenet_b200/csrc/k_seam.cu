@@ -92,130 +92,280 @@ struct Vec<__nv_bfloat16, 8> {
   }
 };
 
+// Asynchronous copies of a thread's own values to its own shared memory, which it alone reads: no barrier, and the loads of the
+// next token are in flight while this one is worked on without a register held for them.  Zeros where `on` is false.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from, bool on) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(on ? 16 : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(smem_u32(to)), "l"(from), "n"(BYTES), "r"(on ? BYTES : 0) : "memory");
+}
+__device__ __forceinline__ void copy_pieces(void* to, const void* from, int bytes) {          // 16 bytes or fewer, zeros behind
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // The gate's factor.  ex2.approx and the approximate reciprocal are good to 2 units in the last place; the product before them
 // loses |g| . 2^-24, so a sigmoid is off by 1e-6 of itself at |g| = 10.
 __device__ __forceinline__ float gate_of(float g, int act) { return act ? __fdividef(1.f, 1.f + __expf(-g)) : g; }
+// the same for a gate of an image, of which there are few: to the last place
+__device__ __forceinline__ float image_gate_of(float g, int act) { return act ? 1.f / (1.f + expf(-g)) : g; }
 // its derivative, from the factor
 __device__ __forceinline__ float gate_slope(float s, int act) { return act ? s * (1.f - s) : 1.f; }
 
 // ------------------------------------------------------------------ channels_first, forward
-// block: 32 x S threads; thread (lane, s) holds channels s CPT .. of pixels 32 VEC tile + VEC lane ..
-// `red`: 2 x S x 32 VEC pairs
+// The VEC pixels of a thread: neighbours, read and written as vectors (ALONG), where rows are aligned to them; else 32 apart.
+// `live`: bit j for a pixel j inside the image (neighbours: all or none).
+template <int VEC, bool ALONG>
+struct Pixels {
+  long long first;
+  unsigned live;
+  __device__ __forceinline__ Pixels(unsigned tile, int lane, long long HW) {
+    first = (long long)tile * (32 * VEC) + (ALONG ? lane * VEC : lane);
+    if (ALONG) {
+      live = first < HW ? (1u << VEC) - 1 : 0u;
+    } else {
+      live = 0;
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) live |= (first + 32 * j < HW ? 1u : 0u) << j;
+    }
+  }
+  // zeros outside
+  template <typename IO>
+  __device__ __forceinline__ void load(const void* p, long long at, float* v, bool on = true) const {
+    if (ALONG) {
+      if (live && on) {
+        Vec<IO, VEC>::load(p, at, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        v[j] = 0.f;
+        if (on && (live >> j & 1)) Vec<IO, 1>::load(p, at + 32 * j, v + j);
+      }
+    }
+  }
+  // The same through shared memory: `fetch` begins it, `fetched` reads it.  Vectors and 4-byte values: a thread's own, which it alone
+  // reads.  Else, 2 bytes being too few for a copy, the warp's pixels of the row in the 16-byte pieces that they lie in (the warp
+  // meets before it reads them and before the next ones come).  `row`: the tile's first pixel; of the bytes before it only those
+  // inside the tensor, from `all` on, are read.
+  template <typename IO>
+  static constexpr bool kOwn = sizeof(IO) == 4 || (ALONG && VEC * sizeof(IO) >= 4);
+  template <typename IO>
+  static constexpr int kSlot = kOwn<IO> ? 32 * VEC * (int)sizeof(IO) : 32 * VEC * (int)sizeof(IO) + 16;          // bytes of a warp
+  template <typename IO>
+  __device__ __forceinline__ void fetch(char* slot, const IO* all, const IO* row, long long HW) const {
+    const int lane = threadIdx.x & 31, tile_first = ALONG ? lane * VEC : lane;
+    if constexpr (kOwn<IO> && ALONG) {
+      copy_async<VEC * sizeof(IO)>(slot + tile_first * sizeof(IO), live ? row + tile_first : row, live);
+    } else if constexpr (kOwn<IO>) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        const bool on = live >> j & 1;
+        copy_async<4>(slot + (lane + 32 * j) * 4, on ? row + lane + 32 * j : row, on);
+      }
+    } else {
+      const long long left = HW - (first - tile_first);
+      const int count = left < 32 * VEC ? (int)left : 32 * VEC, shift = (int)((size_t)row & 15);
+      const int bytes = shift + count * (int)sizeof(IO);
+      const char* from = (const char*)row - shift;
+#pragma unroll
+      for (int k = 0; k < (32 * VEC * (int)sizeof(IO) + 16) / 512 + 1; ++k) {
+        const int at = (k * 32 + lane) * 16;
+        if (at >= bytes) continue;
+        if (from + at >= (const char*)all) {
+          copy_pieces(slot + at, from + at, bytes - at < 16 ? bytes - at : 16);
+        } else {
+          for (int j = shift; j < 16 && j < bytes; j += sizeof(IO)) *(IO*)(slot + j) = *(const IO*)(from + j);
+        }
+      }
+    }
+  }
+  template <typename IO>
+  __device__ __forceinline__ void fetched(const char* slot, const IO* row, float* v) const {
+    const int lane = threadIdx.x & 31;
+    if constexpr (kOwn<IO> && ALONG) {
+      Vec<IO, VEC>::load(slot, lane * VEC, v);
+    } else if constexpr (kOwn<IO>) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) Vec<IO, 1>::load(slot, lane + 32 * j, v + j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) {
+        v[j] = 0.f;
+        if (live >> j & 1) Vec<IO, 1>::load(slot + ((size_t)row & 15), (ALONG ? lane * VEC + j : lane + 32 * j), v + j);
+      }
+    }
+  }
+  template <typename IO>
+  __device__ __forceinline__ void store(void* p, long long at, const float* v) const {
+    if (ALONG) {
+      if (live) Vec<IO, VEC>::store(p, at, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j)
+        if (live >> j & 1) Vec<IO, 1>::store(p, at + 32 * j, v + j);
+    }
+  }
+};
+// block: 32 x S threads; thread (lane, s) holds channels s CPT .. of its pixels of the tile (of 32 VEC)
+// Shared memory: vectors of the channels, padded to CPT; a pair of sums of each warp for each pixel; a pair for each pixel.
+__host__ __device__ inline size_t cf_smem(int S, int CPT, int VEC, int vectors) {
+  return (size_t)vectors * S * CPT * sizeof(float) + (S > 1 ? (size_t)(S + 1) * 32 * VEC * sizeof(float2) : 0);
+}
+// What a branch's normalised value is multiplied by and what is added to it on the way to y (without a gate for each element):
+// scale . s(gate of the image) . (post_w, post_b).  Behind the last channel 0.
+__device__ __forceinline__ float2 branch_factors(const Params& P, int c, long long image) {
+  if (c >= P.C) return make_float2(0.f, 0.f);
+  float a = P.scale ? P.scale[c] : 1.f;
+  if (P.gate_kind == kGateImage) a *= image_gate_of(((const float*)P.gate)[image * P.C + c], P.act);
+  return make_float2(P.post_w ? a * P.post_w[c] : a, P.post_b ? a * P.post_b[c] : 0.f);
+}
+__device__ __forceinline__ void four_of(const float* v, float (&out)[4]) {
+  const float4 q = *(const float4*)v;
+  out[0] = q.x; out[1] = q.y; out[2] = q.z; out[3] = q.w;
+}
+// Mean and 1 / spread of each pixel.  A thread brings the sum of its channels and the squares around their own mean; joined,
+// M2 = sum (M2_i + (sum_i - n_i mean)^2 / n_i).  Values behind the last channel are 0.
 template <int CPT, int VEC>
 __device__ __forceinline__ void cf_stats(const float (&v)[CPT][VEC], int n, const Params& P, float2* red, float (&mean)[VEC],
                                          float (&rstd)[VEC]) {
   const int lane = threadIdx.x & 31, s = threadIdx.x >> 5, S = blockDim.x >> 5;
-  // this thread's mean and squares around it; joined: M2 = sum (M2_i + n_i (m_i - mean)^2)
-  float2 own[VEC];
+  const float inv = 1.f / (float)P.C;
+  float m[VEC], q[VEC];
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) {
-    float m = 0.f, q = 0.f;
-    if (!P.rms) {
+  for (int j = 0; j < VEC; ++j) m[j] = q[j] = 0.f;
+  if (!P.rms) {
+    const float own = 1.f / (float)n;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) m[j] += v[i][j];
+      const float c = m[j] * own;
 #pragma unroll
       for (int i = 0; i < CPT; ++i)
-        if (i < n) m += v[i][j];
-      m = n ? m / (float)n : 0.f;
+        if (i < n) q[j] = fmaf(v[i][j] - c, v[i][j] - c, q[j]);
+      if (S == 1) m[j] = c;
     }
+  } else {
 #pragma unroll
-    for (int i = 0; i < CPT; ++i)
-      if (i < n) q = fmaf(v[i][j] - m, v[i][j] - m, q);
-    own[j] = make_float2(m, q);
+    for (int j = 0; j < VEC; ++j)
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) q[j] = fmaf(v[i][j], v[i][j], q[j]);
   }
-  const float inv = 1.f / (float)P.C;
   if (S == 1) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) mean[j] = own[j].x, rstd[j] = rsqrtf(fmaf(own[j].y, inv, P.eps));
+    for (int j = 0; j < VEC; ++j) mean[j] = m[j], rstd[j] = rsqrtf(fmaf(q[j], inv, P.eps));
     return;
   }
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) red[(s * VEC + j) * 32 + lane] = own[j];
+  for (int j = 0; j < VEC; ++j) red[(s * VEC + j) * 32 + lane] = make_float2(m[j], q[j]);
+  __syncthreads();
+  float2* joined = red + S * VEC * 32;
+  for (int p = threadIdx.x; p < 32 * VEC; p += blockDim.x) {
+    float t = 0.f, u = 0.f;
+    for (int r = 0; r < S; ++r) {
+      const float2 o = red[r * VEC * 32 + p];
+      t += o.x;
+      u += o.y;
+    }
+    t *= inv;
+    if (!P.rms) {
+      for (int r = 0; r < S - 1; ++r) {
+        const float d = fmaf(-(float)CPT, t, red[r * VEC * 32 + p].x);
+        u = fmaf(d * d, 1.f / (float)CPT, u);
+      }
+      const float k = (float)(P.C - (S - 1) * CPT), d = fmaf(-k, t, red[(S - 1) * VEC * 32 + p].x);
+      u += d * d / k;
+    }
+    joined[p] = make_float2(t, rsqrtf(fmaf(u, inv, P.eps)));
+  }
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < VEC; ++j) {
-    float m = 0.f, q = 0.f;
-    if (!P.rms) {
-      for (int t = 0; t < S; ++t) m = fmaf(red[(t * VEC + j) * 32 + lane].x, (float)min(CPT, P.C - t * CPT), m);
-      m *= inv;
-    }
-    for (int t = 0; t < S; ++t) {
-      const float2 o = red[(t * VEC + j) * 32 + lane];
-      q += o.y;
-      if (!P.rms) q = fmaf((o.x - m) * (o.x - m), (float)min(CPT, P.C - t * CPT), q);
-    }
-    mean[j] = m;
-    rstd[j] = rsqrtf(fmaf(q, inv, P.eps));
+    const float2 o = joined[j * 32 + lane];
+    mean[j] = o.x;
+    rstd[j] = o.y;
   }
 }
 
-template <typename IO, int CPT, int VEC, int MAXT>
-__global__ void __launch_bounds__(MAXT) cf_fwd_kernel(const __grid_constant__ Params P) {
+template <typename IO, int CPT, int VEC, bool ALONG, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) cf_fwd_kernel(const __grid_constant__ Params P) {
   pdl_start();
-  extern __shared__ float2 red[];
-  const int lane = threadIdx.x & 31, s = threadIdx.x >> 5, S = blockDim.x >> 5;
+  extern __shared__ __align__(16) float cf_shared[];
+  const int lane = threadIdx.x & 31, s = threadIdx.x >> 5, S = blockDim.x >> 5, padded = S * CPT;
+  float *wy = cf_shared, *oy = wy + padded, *pw = oy + padded, *po = pw + padded;
+  float2* red = (float2*)(po + padded);
   const int c0 = s * CPT, n = min(CPT, P.C - c0);
-  const long long b = blockIdx.x / P.tiles, px = ((long long)(blockIdx.x - b * P.tiles) * 32 + lane) * VEC;
-  const bool live = px < P.HW;
-  const long long base = ((long long)b * P.C + c0) * P.HW + px, token = b * P.HW + px;
+  const long long b = blockIdx.x / P.tiles;
+  const Pixels<VEC, ALONG> px(blockIdx.x - b * P.tiles, lane, P.HW);
+  const long long base = (b * P.C + c0) * P.HW + px.first, token = b * P.HW + px.first;
   float v[CPT][VEC], x[CPT][VEC];
 #pragma unroll
   for (int i = 0; i < CPT; ++i) {
-    if (live && i < n) {
-      Vec<IO, VEC>::load(P.branch, base + i * P.HW, v[i]);
-      Vec<IO, VEC>::load(P.x, base + i * P.HW, x[i]);
+    px.template load<IO>(P.branch, base + i * P.HW, v[i], i < n);
+    px.template load<IO>(P.x, base + i * P.HW, x[i], i < n);
+  }
+  for (int c = threadIdx.x; c < padded; c += blockDim.x) {
+    const float2 f = branch_factors(P, c, b);
+    wy[c] = f.x;
+    oy[c] = f.y;
+    pw[c] = P.pre_w && c < P.C ? P.pre_w[c] : 0.f;
+    po[c] = P.pre_b && c < P.C ? P.pre_b[c] : 0.f;
+  }
+  float mean[VEC], rstd[VEC], w[4], o[4];
+  if (P.post_w) {
+    if (S == 1) __syncthreads();
+    cf_stats<CPT, VEC>(v, n, P, red, mean, rstd);
+    if (P.stats && s == 0) {
+      px.template store<float>(P.stats, token, mean);
+      px.template store<float>(P.stats + P.tokens, token, rstd);
+    }
+#pragma unroll
+    for (int i = 0; i < CPT; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[i][j] = (v[i][j] - mean[j]) * rstd[j];
+  } else {
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < CPT; ++i) {
+    if (i % 4 == 0) four_of(wy + c0 + i, w), four_of(oy + c0 + i, o);
+    if (P.gate_kind == kGateFull) {
+      float g[VEC];
+      px.template load<IO>(P.gate, base + i * P.HW, g, i < n);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[i][j] = fmaf(fmaf(v[i][j], w[i & 3], o[i & 3]), gate_of(g[j], P.act), x[i][j]);
     } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) v[i][j] = x[i][j] = 0.f;
+      for (int j = 0; j < VEC; ++j) v[i][j] = fmaf(v[i][j], w[i & 3], x[i][j] + o[i & 3]);
     }
-  }
-  float mean[VEC], rstd[VEC];
-  if (P.post_w) {
-    cf_stats<CPT, VEC>(v, n, P, red, mean, rstd);
-    if (P.stats && live && s == 0) {
-      Vec<float, VEC>::store(P.stats, token, mean);
-      Vec<float, VEC>::store(P.stats + P.tokens, token, rstd);
-    }
-#pragma unroll
-    for (int i = 0; i < CPT; ++i)
-      if (i < n) {
-        const float w = P.post_w[c0 + i], o = P.post_b ? P.post_b[c0 + i] : 0.f;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i][j] = fmaf((v[i][j] - mean[j]) * rstd[j], w, o);
-      }
-  }
-  if (P.gate_kind == kGateFull && live) {
-#pragma unroll
-    for (int i = 0; i < CPT; ++i)
-      if (i < n) {
-        float g[VEC];
-        Vec<IO, VEC>::load(P.gate, base + i * P.HW, g);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i][j] *= gate_of(g[j], P.act);
-      }
-  }
-#pragma unroll
-  for (int i = 0; i < CPT; ++i)
     if (i < n) {
-      float a = P.scale ? P.scale[c0 + i] : 1.f;
-      if (P.gate_kind == kGateImage) a *= gate_of(((const float*)P.gate)[b * P.C + c0 + i], P.act);
+      px.template store<IO>(P.y, base + i * P.HW, v[i]);
+    } else {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) v[i][j] = fmaf(v[i][j], a, x[i][j]);
-      if (live) Vec<IO, VEC>::store(P.y, base + i * P.HW, v[i]);
+      for (int j = 0; j < VEC; ++j) v[i][j] = 0.f;
     }
+  }
   if (!P.pre_w) return;
-  cf_stats<CPT, VEC>(v, n, P, red + S * 32 * VEC, mean, rstd);
-  if (P.stats && live && s == 0) {
-    Vec<float, VEC>::store(P.stats + 2 * P.tokens, token, mean);
-    Vec<float, VEC>::store(P.stats + 3 * P.tokens, token, rstd);
+  cf_stats<CPT, VEC>(v, n, P, red, mean, rstd);
+  if (P.stats && s == 0) {
+    px.template store<float>(P.stats + 2 * P.tokens, token, mean);
+    px.template store<float>(P.stats + 3 * P.tokens, token, rstd);
   }
-  if (!live) return;
 #pragma unroll
-  for (int i = 0; i < CPT; ++i)
+  for (int i = 0; i < CPT; ++i) {
+    if (i % 4 == 0) four_of(pw + c0 + i, w), four_of(po + c0 + i, o);
     if (i < n) {
-      const float w = P.pre_w[c0 + i], o = P.pre_b ? P.pre_b[c0 + i] : 0.f;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) v[i][j] = fmaf((v[i][j] - mean[j]) * rstd[j], w, o);
-      Vec<IO, VEC>::store(P.z, base + i * P.HW, v[i]);
+      for (int j = 0; j < VEC; ++j) v[i][j] = fmaf((v[i][j] - mean[j]) * rstd[j], w[i & 3], o[i & 3]);
+      px.template store<IO>(P.z, base + i * P.HW, v[i]);
     }
+  }
 }
 
 // Any number of channels: the values are read again for every step (from the L2 cache) instead of being kept.  32 warps.
@@ -226,7 +376,7 @@ __device__ __forceinline__ float cf_sum_value(const Params& P, long long at, int
   Vec<IO, 1>::load(P.x, at, &x);
   if (P.post_w) v = fmaf((v - mean) * rstd, P.post_w[c], P.post_b ? P.post_b[c] : 0.f);
   float a = P.scale ? P.scale[c] : 1.f;
-  if (P.gate_kind == kGateImage) a *= gate_of(((const float*)P.gate)[b * P.C + c], P.act);
+  if (P.gate_kind == kGateImage) a *= image_gate_of(((const float*)P.gate)[b * P.C + c], P.act);
   if (P.gate_kind == kGateFull) {
     Vec<IO, 1>::load(P.gate, at, &g);
     v *= gate_of(g, P.act);
@@ -295,25 +445,30 @@ __global__ void __launch_bounds__(1024) cf_fwd_wide_kernel(const __grid_constant
 }
 
 // ------------------------------------------------------------------ channels_first, backward
-// The sums over the warps of two values for each pixel.  `buf` alternates: the values of the reduction before the last are read
-// by everybody who arrived at the last one.
+// The sums over the warps of two values for each pixel
 template <int VEC>
-__device__ __forceinline__ void cf_join(float (&a)[VEC], float (&b)[VEC], float2* red, int S, int& buf) {
+__device__ __forceinline__ void cf_join(float (&a)[VEC], float (&b)[VEC], float2* red, int S) {
   if (S == 1) return;
   const int lane = threadIdx.x & 31, s = threadIdx.x >> 5;
-  float2* r = red + buf * S * 32 * VEC;
-  buf ^= 1;
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) r[(s * VEC + j) * 32 + lane] = make_float2(a[j], b[j]);
+  for (int j = 0; j < VEC; ++j) red[(s * VEC + j) * 32 + lane] = make_float2(a[j], b[j]);
+  __syncthreads();
+  float2* joined = red + S * VEC * 32;
+  for (int p = threadIdx.x; p < 32 * VEC; p += blockDim.x) {
+    float2 t = red[p];
+    for (int r = 1; r < S; ++r) {
+      const float2 o = red[r * VEC * 32 + p];
+      t.x += o.x;
+      t.y += o.y;
+    }
+    joined[p] = t;
+  }
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < VEC; ++j) {
-    a[j] = b[j] = 0.f;
-    for (int t = 0; t < S; ++t) {
-      const float2 o = r[(t * VEC + j) * 32 + lane];
-      a[j] += o.x;
-      b[j] += o.y;
-    }
+    const float2 o = joined[j * 32 + lane];
+    a[j] = o.x;
+    b[j] = o.y;
   }
 }
 __device__ __forceinline__ float warp_sum(float v) {
@@ -323,86 +478,131 @@ __device__ __forceinline__ float warp_sum(float v) {
 }
 
 // `parts` blocks walk over all images' tiles, or over those of an image where the gate has a value for each image
-template <typename IO, int CPT, int VEC, int MAXT, int MINB>
+template <typename IO, int CPT, int VEC, bool ALONG, bool GATED, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) cf_bwd_kernel(const __grid_constant__ Params P) {
   pdl_start();
-  extern __shared__ float2 red[];
-  const int lane = threadIdx.x & 31, s = threadIdx.x >> 5, S = blockDim.x >> 5;
+  extern __shared__ __align__(16) float cf_shared[];
+  const int lane = threadIdx.x & 31, s = threadIdx.x >> 5, S = blockDim.x >> 5, padded = S * CPT;
+  float *wy = cf_shared, *oy = wy + padded, *pw = oy + padded;
+  float2* red = (float2*)(pw + padded);
+  using Px = Pixels<VEC, ALONG>;
+  // dz, x, branch, the gate of an element, dy of the next tile: CPT slots each; its means and spreads: four (fp32)
+  constexpr int TENSORS = GATED ? 5 : 4, DY = TENSORS - 1;
+  constexpr int SLOT = Px::template kSlot<IO>, STAT = Px::template kSlot<float>;
+  char* const slots = (char*)(red + (S > 1 ? (S + 1) * 32 * VEC : 0)) + s * (TENSORS * CPT * SLOT + 4 * STAT);          // this warp's
+  char* const stats = slots + TENSORS * CPT * SLOT;
   const int c0 = s * CPT, n = min(CPT, P.C - c0);
   const float inv = 1.f / (float)P.C;
   float sa[CPT], sb[CPT], sw[CPT], so[CPT];       // sums A, B; dz k, dz
 #pragma unroll
   for (int i = 0; i < CPT; ++i) sa[i] = sb[i] = sw[i] = so[i] = 0.f;
-  int buf = 0;
   const bool image = P.gate_kind == kGateImage;
-  const long long first = image ? (long long)(blockIdx.x / P.parts) * P.tiles : 0, last = image ? first + P.tiles : (long long)P.tiles * P.B;
-  for (long long tile = first + blockIdx.x % P.parts; tile < last; tile += P.parts) {
-    const long long b = tile / P.tiles, px = ((tile - b * P.tiles) * 32 + lane) * VEC;
-    const bool live = px < P.HW;
-    const long long base = (b * P.C + c0) * P.HW + px, token = b * P.HW + px;
-    float d[CPT][VEC], k[CPT][VEC], h[CPT][VEC], f[CPT][VEC];          // f: the gate
-    float mean[VEC], rstd[VEC], u[VEC], w[VEC];
+  const unsigned of = image ? blockIdx.x / P.parts : 0, first = of * P.tiles, last = image ? first + P.tiles : (unsigned)(P.tiles * P.B);
+  for (int c = threadIdx.x; c < padded; c += blockDim.x) {
+    const float2 f = branch_factors(P, c, of);
+    wy[c] = f.x;
+    oy[c] = f.y;
+    pw[c] = P.pre_w && c < P.C ? P.pre_w[c] : 0.f;
+  }
+  __syncthreads();
+  auto begin = [&](unsigned tile, int from, int to) {
+    if (tile >= last) return;
+    const unsigned b = tile / (unsigned)P.tiles;
+    const Px px(tile - b * P.tiles, lane, P.HW);
+    const long long at = ((long long)b * P.C + c0) * P.HW + (long long)(tile - b * P.tiles) * (32 * VEC);
+    const void* all[5] = {P.dz, P.dz ? P.x : nullptr, P.branch, GATED ? P.gate : P.dy, P.dy};
+    __syncwarp();          // (pieces: what was there is read)
 #pragma unroll
-    for (int i = 0; i < CPT; ++i) {
-      const bool on = live && i < n;
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) d[i][j] = h[i][j] = k[i][j] = 0.f, f[i][j] = 1.f;
-      if (on && P.dz) {
-        Vec<IO, VEC>::load(P.dz, base + i * P.HW, d[i]);
-        Vec<IO, VEC>::load(P.x, base + i * P.HW, k[i]);
-      }
-      if (on && P.branch) Vec<IO, VEC>::load(P.branch, base + i * P.HW, h[i]);
-      if (on && P.branch && P.gate_kind == kGateFull) {
-        Vec<IO, VEC>::load(P.gate, base + i * P.HW, f[i]);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) f[i][j] = gate_of(f[i][j], P.act);
-      } else if (image && i < n) {
-        const float g = gate_of(((const float*)P.gate)[b * P.C + c0 + i], P.act);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) f[i][j] = g;
-      }
-    }
-    if (P.post_w) {
-      if (live) {
-        Vec<float, VEC>::load(P.stats, token, mean);
-        Vec<float, VEC>::load(P.stats, P.tokens + token, rstd);
+    for (int a = 0; a < TENSORS; ++a)
+      if (a >= from && a < to && all[a]) {
+        const IO* row = (const IO*)all[a] + at;
 #pragma unroll
         for (int i = 0; i < CPT; ++i)
+          if (i < n) {
+            px.template fetch<IO>(slots + (a * CPT + i) * SLOT, (const IO*)all[a], row, P.HW);
+            row += P.HW;
+          }
+      }
+    if (from == 0 && P.stats) {
+      const float* row = P.stats + (long long)b * P.HW + (long long)(tile - b * P.tiles) * (32 * VEC);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) h[i][j] = (h[i][j] - mean[j]) * rstd[j];
-      } else {
+      for (int a = 0; a < 4; ++a)
+        if (a < 2 ? P.post_w != nullptr : P.dz != nullptr) px.template fetch<float>(stats + a * STAT, P.stats, row + a * P.tokens, P.HW);
+    }
+  };
+  auto get = [&](const Px& px, int a, int i, const void* p, long long row, float (&v)[VEC]) {
+    if (!p || i >= n) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) rstd[j] = 1.f;
+      for (int j = 0; j < VEC; ++j) v[j] = 0.f;
+    } else {
+      px.template fetched<IO>(slots + (a * CPT + i) * SLOT, (const IO*)p + row, v);
+    }
+  };
+  auto stat = [&](const Px& px, int a, long long row, float (&v)[VEC]) {
+    px.template fetched<float>(stats + a * STAT, P.stats + a * P.tokens + row, v);
+  };
+  begin(first + blockIdx.x % P.parts, 0, TENSORS);
+  for (unsigned tile = first + blockIdx.x % P.parts; tile < last; tile += P.parts) {
+    const unsigned b = tile / (unsigned)P.tiles;
+    const Px px(tile - b * P.tiles, lane, P.HW);
+    const long long tile_at = (long long)(tile - b * P.tiles) * (32 * VEC), row = ((long long)b * P.C + c0) * P.HW + tile_at;
+    const long long base = ((long long)b * P.C + c0) * P.HW + px.first, token_row = (long long)b * P.HW + tile_at;
+    float d[CPT][VEC], k[CPT][VEC], h[CPT][VEC], f[GATED ? CPT : 1][VEC];          // f: the gate of an element
+    float mean[VEC], rstd[VEC], u[VEC], w[VEC], vec[4], add[4];
+    copies_done();
+    if (!Px::template kOwn<IO>) __syncwarp();
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) {
+      get(px, 0, i, P.dz, row + i * P.HW, d[i]);
+      get(px, 1, i, P.dz ? P.x : nullptr, row + i * P.HW, k[i]);
+      get(px, 2, i, P.branch, row + i * P.HW, h[i]);
+      if constexpr (GATED) {
+        get(px, 3, i, P.gate, row + i * P.HW, f[i]);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) f[i][j] = gate_of(f[i][j], P.act);
       }
     }
+    float mk[VEC], rk[VEC];
     if (P.dz) {
-      float mk[VEC], rk[VEC];
-      if (live) {
-        Vec<float, VEC>::load(P.stats, 2 * P.tokens + token, mk);
-        Vec<float, VEC>::load(P.stats, 3 * P.tokens + token, rk);
-      } else {
+      stat(px, 2, token_row, mk);
+      stat(px, 3, token_row, rk);
+    }
+    if (P.post_w) {
+      stat(px, 0, token_row, mean);
+      stat(px, 1, token_row, rstd);
+    }
+    begin(tile + P.parts, 0, DY);
+    if (P.post_w) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) mk[j] = 0.f, rk[j] = 1.f;
+      for (int i = 0; i < CPT; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) h[i][j] = i < n ? (h[i][j] - mean[j]) * rstd[j] : 0.f;
+    }
+    if (P.dz) {
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) {
+        if (i % 4 == 0) four_of(wy + c0 + i, vec), four_of(oy + c0 + i, add);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)          // y again, as it was before it was rounded
+          k[i][j] = (GATED ? fmaf(fmaf(h[i][j], vec[i & 3], add[i & 3]), f[GATED ? i : 0][j], k[i][j])
+                           : fmaf(h[i][j], vec[i & 3], k[i][j] + add[i & 3])) - mk[j];
       }
 #pragma unroll
       for (int j = 0; j < VEC; ++j) u[j] = w[j] = 0.f;
 #pragma unroll
-      for (int i = 0; i < CPT; ++i)
-        if (live && i < n) {
-          const float a = P.scale ? P.scale[c0 + i] : 1.f, pw = P.post_w ? P.post_w[c0 + i] : 1.f;
-          const float pb = P.post_b ? P.post_b[c0 + i] : 0.f, g = P.pre_w[c0 + i];
+      for (int i = 0; i < CPT; ++i) {
+        if (i % 4 == 0) four_of(pw + c0 + i, vec);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            // y again, as it was before it was rounded
-            k[i][j] = (fmaf(fmaf(h[i][j], pw, pb) * f[i][j], a, k[i][j]) - mk[j]) * rk[j];
-            so[i] += d[i][j];
-            sw[i] = fmaf(d[i][j], k[i][j], sw[i]);
-            d[i][j] *= g;
-            u[j] += d[i][j];
-            w[j] = fmaf(d[i][j], k[i][j], w[j]);
-          }
+        for (int j = 0; j < VEC; ++j) {        // (dz is 0 behind the last pixel and channel, and so are the sums)
+          k[i][j] *= rk[j];
+          so[i] += d[i][j];
+          sw[i] = fmaf(d[i][j], k[i][j], sw[i]);
+          d[i][j] *= vec[i & 3];
+          u[j] += d[i][j];
+          w[j] = fmaf(d[i][j], k[i][j], w[j]);
         }
-      cf_join<VEC>(u, w, red, S, buf);
+      }
+      cf_join<VEC>(u, w, red, S);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         u[j] = P.rms ? 0.f : u[j] * inv;
@@ -411,46 +611,56 @@ __global__ void __launch_bounds__(MAXT, MINB) cf_bwd_kernel(const __grid_constan
 #pragma unroll
       for (int i = 0; i < CPT; ++i)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) d[i][j] = rk[j] * (d[i][j] - u[j] - k[i][j] * w[j]);
+        for (int j = 0; j < VEC; ++j) d[i][j] = rk[j] * (d[i][j] - fmaf(k[i][j], w[j], u[j]));
     }
 #pragma unroll
-    for (int i = 0; i < CPT; ++i)
-      if (live && i < n) {
-        if (P.dy) {
-          float e[VEC];
-          Vec<IO, VEC>::load(P.dy, base + i * P.HW, e);
+    for (int i = 0; i < CPT; ++i) {
+      if (P.dy) {
+        float e[VEC];
+        get(px, DY, i, P.dy, row + i * P.HW, e);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) d[i][j] += e[j];
-        }
-        if (P.dx) Vec<IO, VEC>::store(P.dx, base + i * P.HW, d[i]);
+        for (int j = 0; j < VEC; ++j) d[i][j] += e[j];
       }
+      if (i < n) {
+        if (P.dx) px.template store<IO>(P.dx, base + i * P.HW, d[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) d[i][j] = 0.f;
+      }
+    }
+    begin(tile + P.parts, DY, TENSORS);
     if (!P.branch) continue;
+    if constexpr (GATED) {
+#pragma unroll
+      for (int i = 0; i < CPT; ++i) {
+        if (i % 4 == 0) four_of(wy + c0 + i, vec), four_of(oy + c0 + i, add);
+        if (i < n && P.dgate) {
+          float dg[VEC];
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) dg[j] = d[i][j] * fmaf(h[i][j], vec[i & 3], add[i & 3]) * gate_slope(f[i][j], P.act);
+          px.template store<IO>(P.dgate, base + i * P.HW, dg);
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) d[i][j] *= f[i][j];
+      }
+    }
 #pragma unroll
     for (int j = 0; j < VEC; ++j) u[j] = w[j] = 0.f;
 #pragma unroll
-    for (int i = 0; i < CPT; ++i)
-      if (live && i < n) {
-        const float a = P.scale ? P.scale[c0 + i] : 1.f, pw = P.post_w ? P.post_w[c0 + i] : 1.f;
-        if (P.gate_kind == kGateFull && P.dgate) {
-          const float pb = P.post_b ? P.post_b[c0 + i] : 0.f;
-          float dg[VEC];
+    for (int i = 0; i < CPT; ++i) {
+      if (i % 4 == 0) four_of(wy + c0 + i, vec);
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) dg[j] = d[i][j] * a * fmaf(h[i][j], pw, pb) * gate_slope(f[i][j], P.act);
-          Vec<IO, VEC>::store(P.dgate, base + i * P.HW, dg);
-        }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          if (!image) d[i][j] *= f[i][j];          // (an image's sums are without its gate)
-          sb[i] += d[i][j];
-          sa[i] = fmaf(d[i][j], h[i][j], sa[i]);
-          d[i][j] *= image ? a * pw * f[i][j] : a * pw;
-          u[j] += d[i][j];
-          w[j] = fmaf(d[i][j], h[i][j], w[j]);
-        }
+      for (int j = 0; j < VEC; ++j) {          // (an image's sums are without its gate, which is in vec)
+        sb[i] += d[i][j];
+        sa[i] = fmaf(d[i][j], h[i][j], sa[i]);
+        d[i][j] *= vec[i & 3];
+        u[j] += d[i][j];
+        w[j] = fmaf(d[i][j], h[i][j], w[j]);
       }
+    }
     if (!P.dbranch) continue;
     if (P.post_w) {
-      cf_join<VEC>(u, w, red, S, buf);
+      cf_join<VEC>(u, w, red, S);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         u[j] = P.rms ? 0.f : u[j] * inv;
@@ -459,14 +669,15 @@ __global__ void __launch_bounds__(MAXT, MINB) cf_bwd_kernel(const __grid_constan
     }
 #pragma unroll
     for (int i = 0; i < CPT; ++i)
-      if (live && i < n) {
+      if (i < n) {
         if (P.post_w) {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) d[i][j] = rstd[j] * (d[i][j] - u[j] - h[i][j] * w[j]);
+          for (int j = 0; j < VEC; ++j) d[i][j] = rstd[j] * (d[i][j] - fmaf(h[i][j], w[j], u[j]));
         }
-        Vec<IO, VEC>::store(P.dbranch, base + i * P.HW, d[i]);
+        px.template store<IO>(P.dbranch, base + i * P.HW, d[i]);
       }
   }
+  copies_done();
   if (!P.partial) return;
   float* out = P.partial + (long long)blockIdx.x * 4 * P.C;
 #pragma unroll
@@ -531,7 +742,7 @@ __global__ void __launch_bounds__(1024) cf_bwd_wide_kernel(const __grid_constant
     };
     auto factor = [&](int c, float g) {    // what takes it to the normalised branch
       float a = P.scale ? P.scale[c] : 1.f;
-      if (image) a *= gate_of(((const float*)P.gate)[b * P.C + c], P.act);
+      if (image) a *= image_gate_of(((const float*)P.gate)[b * P.C + c], P.act);
       if (P.gate_kind == kGateFull) a *= g;
       return P.post_w ? a * P.post_w[c] : a;
     };
@@ -585,34 +796,33 @@ __global__ void __launch_bounds__(1024) cf_bwd_wide_kernel(const __grid_constant
 
 // ------------------------------------------------------------------ channels_last
 // `tpr` threads (a power of two) share a token: thread t holds the vectors t, t + tpr, ... of its channels.
-// Sum over the token's threads; `red`: the block's, for tokens of more than a warp.
-__device__ __forceinline__ float cl_sum(float v, int tpr, float* red) {
-  for (int o = (tpr < 32 ? tpr : 32) >> 1; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (tpr <= 32) return v;
-  __syncthreads();          // the values before are read
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.f;
-  const int w0 = (threadIdx.x & ~(tpr - 1)) >> 5;
-  for (int j = 0; j < (tpr >> 5); ++j) v += red[w0 + j];
-  return v;
-}
-__device__ __forceinline__ float2 cl_sum2(float2 v, int tpr, float2* red) {
-  for (int o = (tpr < 32 ? tpr : 32) >> 1; o; o >>= 1) {
-    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+// Sums over the token's threads.  Tokens of more than a warp meet in `red` (twice 32 values of the block): `buf` alternates, since
+// the values of the sum before the last have been read by everybody who arrived at the last one.
+template <int N>
+__device__ __forceinline__ void cl_sum(float (&v)[N], int tpr, float2* red, int& buf) {
+  if (tpr >= 32) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1)
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] += __shfl_xor_sync(0xffffffffu, v[j], o);
+  } else {
+    for (int o = tpr >> 1; o; o >>= 1)
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] += __shfl_xor_sync(0xffffffffu, v[j], o);
   }
-  if (tpr <= 32) return v;
+  if (tpr <= 32) return;
+  float2* r = red + 32 * buf;
+  buf ^= 1;
+  if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = make_float2(v[0], v[N - 1]);
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = make_float2(0.f, 0.f);
-  const int w0 = (threadIdx.x & ~(tpr - 1)) >> 5;
-  for (int j = 0; j < (tpr >> 5); ++j) v.x += red[w0 + j].x, v.y += red[w0 + j].y;
-  return v;
+  r += (threadIdx.x & ~(tpr - 1)) >> 5;
+  float2 t = r[0];
+  for (int j = 1; j < (tpr >> 5); ++j) t.x += r[j].x, t.y += r[j].y;
+  v[0] = t.x;
+  if (N == 2) v[1] = t.y;
 }
 template <int NV, int V>
-__device__ __forceinline__ void cl_stats(const float (&v)[NV][V], const Params& P, int tpr, int t, float* red, float& mean,
+__device__ __forceinline__ void cl_stats(const float (&v)[NV][V], const Params& P, int tpr, int t, float2* red, int& buf, float& mean,
                                          float& rstd) {
   const float inv = 1.f / (float)P.C;
   float m = 0.f, q = 0.f;
@@ -622,7 +832,9 @@ __device__ __forceinline__ void cl_stats(const float (&v)[NV][V], const Params& 
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < V; ++j) m += v[i][j];          // (zeros behind the last channel)
-    mean = cl_sum(m, tpr, red) * inv;
+    float all[1] = {m};
+    cl_sum(all, tpr, red, buf);
+    mean = all[0] * inv;
   }
 #pragma unroll
   for (int i = 0; i < NV; ++i)
@@ -630,7 +842,9 @@ __device__ __forceinline__ void cl_stats(const float (&v)[NV][V], const Params& 
 #pragma unroll
       for (int j = 0; j < V; ++j) q = fmaf(v[i][j] - mean, v[i][j] - mean, q);
     }
-  rstd = rsqrtf(fmaf(cl_sum(q, tpr, red), inv, P.eps));
+  float all[1] = {q};
+  cl_sum(all, tpr, red, buf);
+  rstd = rsqrtf(fmaf(all[0], inv, P.eps));
 }
 template <int V>
 __device__ __forceinline__ void cl_vector(const float* p, int c, float other, float (&v)[V]) {
@@ -647,182 +861,247 @@ __device__ __forceinline__ void cl_vector(const float* p, int c, float other, fl
   }
 }
 
-template <typename IO, int NV, int V, int MAXT>
-__global__ void __launch_bounds__(MAXT) cl_fwd_kernel(const __grid_constant__ Params P) {
+// the factors of branch_factors for V channels (a gate of each image apart)
+template <int V>
+__device__ __forceinline__ void cl_factors(const Params& P, int c, float (&w)[V], float (&o)[V]) {
+  float a[V];
+  cl_vector<V>(P.scale, c, 1.f, a);
+  cl_vector<V>(P.post_w, c, 1.f, w);
+  cl_vector<V>(P.post_b, c, 0.f, o);
+#pragma unroll
+  for (int j = 0; j < V; ++j) w[j] *= a[j], o[j] *= a[j];
+}
+
+// Blocks walk over tokens with the vectors of their channels in registers; the next token's values are loaded before this one's
+// norms are known.
+template <typename IO, int NV, int V, int MAXT, int MINB>
+__global__ void __launch_bounds__(MAXT, MINB) cl_fwd_kernel(const __grid_constant__ Params P) {
   pdl_start();
-  __shared__ float red[32];
+  __shared__ float2 red[64];
+  int buf = 0;
   const int tpr = P.tpr, t = threadIdx.x & (tpr - 1), rows = blockDim.x / tpr;
-  const long long token = (long long)blockIdx.x * rows + threadIdx.x / tpr;
-  const bool live = token < P.tokens;
-  const long long base = token * P.C, b = live ? token / P.HW : 0;
-  float v[NV][V], x[NV][V];
+  float wy[NV][V], oy[NV][V], pw[NV][V], po[NV][V], v[NV][V], x[NV][V];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * tpr + t) * V;
-    if (live && c < P.C) {
-      Vec<IO, V>::load(P.branch, base + c, v[i]);
-      Vec<IO, V>::load(P.x, base + c, x[i]);
-    } else {
 #pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] = x[i][j] = 0.f;
-    }
-  }
-  float mean = 0.f, rstd = 1.f;
-  if (P.post_w) {
-    cl_stats<NV, V>(v, P, tpr, t, red, mean, rstd);
-    if (P.stats && live && t == 0) P.stats[token] = mean, P.stats[P.tokens + token] = rstd;
-  }
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * tpr + t) * V;
-    if (c >= P.C || !live) continue;
-    float w[V], o[V];
-    if (P.post_w) {
-      cl_vector<V>(P.post_w, c, 1.f, w);
-      cl_vector<V>(P.post_b, c, 0.f, o);
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] = fmaf((v[i][j] - mean) * rstd, w[j], o[j]);
-    }
-    if (P.gate_kind) {
-      if (P.gate_kind == kGateFull) Vec<IO, V>::load(P.gate, base + c, w);
-      else cl_vector<V>((const float*)P.gate + b * P.C, c, 0.f, w);
-#pragma unroll
-      for (int j = 0; j < V; ++j) v[i][j] *= gate_of(w[j], P.act);
-    }
-    cl_vector<V>(P.scale, c, 1.f, w);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[i][j] = fmaf(v[i][j], w[j], x[i][j]);
-    Vec<IO, V>::store(P.y, base + c, v[i]);
-  }
-  if (!P.pre_w) return;
-  cl_stats<NV, V>(v, P, tpr, t, red, mean, rstd);
-  if (!live) return;
-  if (P.stats && t == 0) P.stats[2 * P.tokens + token] = mean, P.stats[3 * P.tokens + token] = rstd;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int c = (i * tpr + t) * V;
+    for (int j = 0; j < V; ++j) wy[i][j] = oy[i][j] = pw[i][j] = po[i][j] = 0.f;
     if (c >= P.C) continue;
-    float w[V], o[V];
-    cl_vector<V>(P.pre_w, c, 1.f, w);
-    cl_vector<V>(P.pre_b, c, 0.f, o);
+    cl_factors<V>(P, c, wy[i], oy[i]);
+    if (P.pre_w) {
+      cl_vector<V>(P.pre_w, c, 1.f, pw[i]);
+      cl_vector<V>(P.pre_b, c, 0.f, po[i]);
+    }
+  }
+  auto fetch = [&](long long token) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[i][j] = fmaf((v[i][j] - mean) * rstd, w[j], o[j]);
-    Vec<IO, V>::store(P.z, base + c, v[i]);
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * tpr + t) * V;
+      if (token < P.tokens && c < P.C) {
+        Vec<IO, V>::load(P.branch, token * P.C + c, v[i]);
+        Vec<IO, V>::load(P.x, token * P.C + c, x[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[i][j] = x[i][j] = 0.f;
+      }
+    }
+  };
+  const long long step = (long long)gridDim.x * rows;
+  long long start = (long long)blockIdx.x * rows;
+  fetch(start + threadIdx.x / tpr);
+  for (; start < P.tokens; start += step) {
+    const long long token = start + threadIdx.x / tpr, base = token * P.C;
+    const bool live = token < P.tokens;
+    float mean = 0.f, rstd = 1.f, y[NV][V];
+    if (P.post_w) {
+      cl_stats<NV, V>(v, P, tpr, t, red, buf, mean, rstd);
+      if (P.stats && live && t == 0) P.stats[token] = mean, P.stats[P.tokens + token] = rstd;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * tpr + t) * V;
+      float g[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) y[i][j] = fmaf((v[i][j] - mean) * rstd, wy[i][j], oy[i][j]);
+      if (c < P.C && live) {
+        if (P.gate_kind) {
+          if (P.gate_kind == kGateFull) Vec<IO, V>::load(P.gate, base + c, g);
+          else cl_vector<V>((const float*)P.gate + token / P.HW * P.C, c, 0.f, g);
+#pragma unroll
+          for (int j = 0; j < V; ++j) y[i][j] *= gate_of(g[j], P.act);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) y[i][j] += x[i][j];
+        Vec<IO, V>::store(P.y, base + c, y[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) y[i][j] = 0.f;
+      }
+    }
+    fetch(token + step);
+    if (!P.pre_w) continue;
+    cl_stats<NV, V>(y, P, tpr, t, red, buf, mean, rstd);
+    if (!live) continue;
+    if (P.stats && t == 0) P.stats[2 * P.tokens + token] = mean, P.stats[3 * P.tokens + token] = rstd;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (i * tpr + t) * V;
+      if (c >= P.C) continue;
+#pragma unroll
+      for (int j = 0; j < V; ++j) y[i][j] = fmaf((y[i][j] - mean) * rstd, pw[i][j], po[i][j]);
+      Vec<IO, V>::store(P.z, base + c, y[i]);
+    }
   }
 }
+
+template <typename IO, int NV, int V>
+__host__ __device__ constexpr bool cl_async() { return V * sizeof(IO) >= 4 && NV * V * sizeof(IO) <= 32; }
 
 template <typename IO, int NV, int V, int MAXT, int MINB>
 __global__ void __launch_bounds__(MAXT, MINB) cl_bwd_kernel(const __grid_constant__ Params P) {
   pdl_start();
-  __shared__ float2 red[32];
-  extern __shared__ float2 joined[];          // 4 C floats for each warp, or each token of more than a warp
+  int buf = 0;
+  // 64 pairs for the sums; dz, x, branch, gate, dy of the next token, in the end 4 C floats for each warp, or each token of more than a
+  // warp
+  extern __shared__ __align__(16) char cl_dynamic[];
+  float2* const red = (float2*)cl_dynamic;
+  char* const cl_shared = cl_dynamic + 64 * sizeof(float2);
+  constexpr int BYTES = V * sizeof(IO), SLOT = MAXT * BYTES;
+  constexpr bool ASYNC = cl_async<IO, NV, V>();
   const int tpr = P.tpr, t = threadIdx.x & (tpr - 1), rows = blockDim.x / tpr, row = threadIdx.x / tpr;
   const float inv = 1.f / (float)P.C;
   const bool image = P.gate_kind == kGateImage;
   const long long of = blockIdx.x / P.parts, first = image ? of * P.HW : 0, last = image ? first + P.HW : P.tokens;
-  float sa[NV][V], sb[NV][V], sw[NV][V], so[NV][V];
+  float sa[NV][V], sb[NV][V], sw[NV][V], so[NV][V], wy[NV][V], oy[NV][V], pw[NV][V];
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    const int c = (i * tpr + t) * V;
 #pragma unroll
-    for (int j = 0; j < V; ++j) sa[i][j] = sb[i][j] = sw[i][j] = so[i][j] = 0.f;
-  for (long long start = first + (long long)(blockIdx.x % P.parts) * rows; start < last; start += (long long)P.parts * rows) {
+    for (int j = 0; j < V; ++j) sa[i][j] = sb[i][j] = sw[i][j] = so[i][j] = wy[i][j] = oy[i][j] = pw[i][j] = 0.f;
+    if (c >= P.C) continue;
+    cl_factors<V>(P, c, wy[i], oy[i]);
+    if (P.pre_w) cl_vector<V>(P.pre_w, c, 1.f, pw[i]);
+    if (image) {
+      float g[V];
+      cl_vector<V>((const float*)P.gate + of * P.C, c, 0.f, g);
+#pragma unroll
+      for (int j = 0; j < V; ++j) g[j] = image_gate_of(g[j], P.act), wy[i][j] *= g[j], oy[i][j] *= g[j];
+    }
+  }
+  const long long step = (long long)P.parts * rows;
+  long long start = first + (long long)(blockIdx.x % P.parts) * rows;
+  float stat[4];          // means and spreads of the next token
+  auto begin = [&](long long token) {
+    const bool live = token < last;
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      stat[a] = a & 1 ? 1.f : 0.f;
+      if (live && (a < 2 ? P.post_w != nullptr : P.dz != nullptr)) stat[a] = P.stats[a * P.tokens + token];
+    }
+    if constexpr (ASYNC) {
+      const void* all[5] = {P.dz, P.dz ? P.x : nullptr, P.branch, P.gate_kind == kGateFull ? P.gate : nullptr, P.dy};
+#pragma unroll
+      for (int a = 0; a < 5; ++a)
+        if (all[a]) {
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            const int c = (i * tpr + t) * V;
+            const bool on = live && c < P.C;
+            copy_async<BYTES>(cl_shared + (a * NV + i) * SLOT + threadIdx.x * BYTES, (const IO*)all[a] + (on ? token * P.C + c : 0), on);
+          }
+        }
+    }
+  };
+  auto get = [&](int a, int i, const void* p, long long at, bool on, float (&v)[V]) {
+    if (!p || !on) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = 0.f;
+    } else if constexpr (ASYNC) {
+      Vec<IO, V>::load(cl_shared + (a * NV + i) * SLOT, threadIdx.x * V, v);
+    } else {
+      Vec<IO, V>::load(p, at, v);
+    }
+  };
+  begin(start + row);
+  for (; start < last; start += step) {
     const long long token = start + row;
     const bool live = token < last;
     const long long base = token * P.C;
-    float d[NV][V], k[NV][V], h[NV][V], f[NV][V];          // f: the gate
-    float mean = 0.f, rstd = 1.f;
-    if (P.post_w && live) mean = P.stats[token], rstd = P.stats[P.tokens + token];
+    float d[NV][V], k[NV][V], h[NV][V], f[NV][V], e[NV][V];          // f: the gate; e: dy
+    const float mean = stat[0], rstd = stat[1], mk = stat[2], rk = stat[3];
+    if (ASYNC) copies_done();
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * tpr + t) * V;
       const bool on = live && c < P.C;
+      get(0, i, P.dz, base + c, on, d[i]);
+      get(1, i, P.dz ? P.x : nullptr, base + c, on, k[i]);
+      get(2, i, P.branch, base + c, on, h[i]);
+      get(4, i, P.dy, base + c, on, e[i]);
 #pragma unroll
-      for (int j = 0; j < V; ++j) d[i][j] = k[i][j] = h[i][j] = 0.f, f[i][j] = 1.f;
-      if (on && P.dz) {
-        Vec<IO, V>::load(P.dz, base + c, d[i]);
-        Vec<IO, V>::load(P.x, base + c, k[i]);
-      }
-      if (on && P.branch) {
-        Vec<IO, V>::load(P.branch, base + c, h[i]);
-#pragma unroll
-        for (int j = 0; j < V; ++j) h[i][j] = (h[i][j] - mean) * rstd;
-      }
-      if (on && P.branch && P.gate_kind) {
-        if (image) cl_vector<V>((const float*)P.gate + of * P.C, c, 0.f, f[i]);
-        else Vec<IO, V>::load(P.gate, base + c, f[i]);
+      for (int j = 0; j < V; ++j) h[i][j] = on ? (h[i][j] - mean) * rstd : 0.f, f[i][j] = 1.f;
+      if (P.gate_kind == kGateFull) {
+        get(3, i, P.gate, base + c, on, f[i]);
 #pragma unroll
         for (int j = 0; j < V; ++j) f[i][j] = gate_of(f[i][j], P.act);
       }
     }
+    begin(token + step);
     if (P.dz) {
-      const float mk = live ? P.stats[2 * P.tokens + token] : 0.f, rk = live ? P.stats[3 * P.tokens + token] : 1.f;
-      float2 u = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = (i * tpr + t) * V;
-        if (c >= P.C || !live) continue;
-        float w[V], a[V], pw[V], pb[V];
-        cl_vector<V>(P.pre_w, c, 1.f, w);
-        cl_vector<V>(P.scale, c, 1.f, a);
-        cl_vector<V>(P.post_w, c, 1.f, pw);
-        cl_vector<V>(P.post_b, c, 0.f, pb);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          // y again, as it was before it was rounded
-          k[i][j] = (fmaf(fmaf(h[i][j], pw[j], pb[j]) * f[i][j], a[j], k[i][j]) - mk) * rk;
-          so[i][j] += d[i][j];
-          sw[i][j] = fmaf(d[i][j], k[i][j], sw[i][j]);
-          d[i][j] *= w[j];
-          u.x += d[i][j];
-          u.y = fmaf(d[i][j], k[i][j], u.y);
-        }
-      }
-      u = cl_sum2(u, tpr, red);
-      u.x = P.rms ? 0.f : u.x * inv;
-      u.y *= inv;
+      float u[2] = {0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[i][j] = rk * (d[i][j] - u.x - k[i][j] * u.y);
+        for (int j = 0; j < V; ++j) {          // (dz is 0 behind the last token and channel, and so are the sums)
+          // y again, as it was before it was rounded
+          k[i][j] = (fmaf(fmaf(h[i][j], wy[i][j], oy[i][j]), f[i][j], k[i][j]) - mk) * rk;
+          so[i][j] += d[i][j];
+          sw[i][j] = fmaf(d[i][j], k[i][j], sw[i][j]);
+          d[i][j] *= pw[i][j];
+          u[0] += d[i][j];
+          u[1] = fmaf(d[i][j], k[i][j], u[1]);
+        }
+      cl_sum(u, tpr, red, buf);
+      u[0] = P.rms ? 0.f : u[0] * inv;
+      u[1] *= inv;
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[i][j] = rk * (d[i][j] - u[0] - k[i][j] * u[1]);
     }
-    float2 u = make_float2(0.f, 0.f);
+    float u[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * tpr + t) * V;
       if (c >= P.C || !live) continue;
-      if (P.dy) {
-        float w[V];
-        Vec<IO, V>::load(P.dy, base + c, w);
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[i][j] += w[j];
-      }
+      for (int j = 0; j < V; ++j) d[i][j] += e[i][j];
       if (P.dx) Vec<IO, V>::store(P.dx, base + c, d[i]);
       if (!P.branch) continue;
-      float a[V], pw[V];
-      cl_vector<V>(P.scale, c, 1.f, a);
-      cl_vector<V>(P.post_w, c, 1.f, pw);
-      if (P.gate_kind == kGateFull && P.dgate) {
-        float o[V];
-        cl_vector<V>(P.post_b, c, 0.f, o);
+      if (P.gate_kind == kGateFull) {
+        if (P.dgate) {
+          float o[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = d[i][j] * a[j] * fmaf(h[i][j], pw[j], o[j]) * gate_slope(f[i][j], P.act);
-        Vec<IO, V>::store(P.dgate, base + c, o);
+          for (int j = 0; j < V; ++j) o[j] = d[i][j] * fmaf(h[i][j], wy[i][j], oy[i][j]) * gate_slope(f[i][j], P.act);
+          Vec<IO, V>::store(P.dgate, base + c, o);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) d[i][j] *= f[i][j];
       }
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (!image) d[i][j] *= f[i][j];          // (an image's sums are without its gate)
+      for (int j = 0; j < V; ++j) {          // (an image's sums are without its gate, which is in wy)
         sb[i][j] += d[i][j];
         sa[i][j] = fmaf(d[i][j], h[i][j], sa[i][j]);
-        d[i][j] *= image ? a[j] * pw[j] * f[i][j] : a[j] * pw[j];
-        u.x += d[i][j];
-        u.y = fmaf(d[i][j], h[i][j], u.y);
+        d[i][j] *= wy[i][j];
+        u[0] += d[i][j];
+        u[1] = fmaf(d[i][j], h[i][j], u[1]);
       }
     }
     if (!P.dbranch) continue;
     if (P.post_w) {
-      u = cl_sum2(u, tpr, red);
-      u.x = P.rms ? 0.f : u.x * inv;
-      u.y *= inv;
+      cl_sum(u, tpr, red, buf);
+      u[0] = P.rms ? 0.f : u[0] * inv;
+      u[1] *= inv;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -830,7 +1109,7 @@ __global__ void __launch_bounds__(MAXT, MINB) cl_bwd_kernel(const __grid_constan
       if (c >= P.C || !live) continue;
       if (P.post_w) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[i][j] = rstd * (d[i][j] - u.x - h[i][j] * u.y);
+        for (int j = 0; j < V; ++j) d[i][j] = rstd * (d[i][j] - u[0] - h[i][j] * u[1]);
       }
       Vec<IO, V>::store(P.dbranch, base + c, d[i]);
     }
@@ -838,7 +1117,10 @@ __global__ void __launch_bounds__(MAXT, MINB) cl_bwd_kernel(const __grid_constan
   if (!P.partial) return;
   float* out = P.partial + (long long)blockIdx.x * 4 * P.C;
   const int slots = blockDim.x / (tpr > 32 ? tpr : 32);
-  float* own = slots > 1 ? (float*)joined + (threadIdx.x / (tpr > 32 ? tpr : 32)) * 4 * P.C : out;
+  float* const joined = (float*)cl_shared;
+  float* own = slots > 1 ? joined + (threadIdx.x / (tpr > 32 ? tpr : 32)) * 4 * P.C : out;
+  if (ASYNC) copies_done();
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int c = (i * tpr + t) * V;
@@ -862,7 +1144,7 @@ __global__ void __launch_bounds__(MAXT, MINB) cl_bwd_kernel(const __grid_constan
   __syncthreads();
   for (int i = threadIdx.x; i < 4 * P.C; i += blockDim.x) {
     float v = 0.f;
-    for (int w = 0; w < slots; ++w) v += ((float*)joined)[w * 4 * P.C + i];
+    for (int w = 0; w < slots; ++w) v += joined[w * 4 * P.C + i];
     out[i] = v;
   }
 }
@@ -871,12 +1153,13 @@ __global__ void __launch_bounds__(MAXT, MINB) cl_bwd_kernel(const __grid_constan
 // grid: (groups of 32 channels, 2): the sums A, B and what follows from them; the sums of dz
 __global__ void __launch_bounds__(1024) finish_kernel(const __grid_constant__ Params P) {
   pdl_start();
-  __shared__ double red[32][32][2];
-  const int lane = threadIdx.x & 31, s = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  __shared__ double red[32][33][2];
+  const int lane = threadIdx.x & 31, s = threadIdx.x >> 5;
+  int c = blockIdx.x * 32 + lane;
   const bool pre = blockIdx.y == 1;
   const int images = P.gate_kind == kGateImage ? (int)P.B : 1;
-  const float a = P.scale && c < P.C ? P.scale[c] : 1.f, w = P.post_w && c < P.C ? P.post_w[c] : 1.f;
-  const float o = P.post_b && c < P.C ? P.post_b[c] : 0.f;
+  float a = P.scale && c < P.C ? P.scale[c] : 1.f, w = P.post_w && c < P.C ? P.post_w[c] : 1.f;
+  float o = P.post_b && c < P.C ? P.post_b[c] : 0.f;
   // `share` of the 32 rows of threads add up an image, the others other images
   int share = 32;
   while (share > 1 && images > 32 / share) share >>= 1;
@@ -902,7 +1185,7 @@ __global__ void __launch_bounds__(1024) finish_kernel(const __grid_constant__ Pa
       if (s % share) u0 = u1 = 0;
     }
     if (P.gate_kind == kGateImage && !pre && c < P.C && b < images && s % share == 0) {
-      const float g = gate_of(((const float*)P.gate)[(long long)b * P.C + c], P.act);
+      const float g = image_gate_of(((const float*)P.gate)[(long long)b * P.C + c], P.act);
       if (P.dgate) ((float*)P.dgate)[(long long)b * P.C + c] = (float)(a * (w * u0 + o * u1) * gate_slope(g, P.act));
       u0 *= g;
       u1 *= g;
@@ -910,12 +1193,22 @@ __global__ void __launch_bounds__(1024) finish_kernel(const __grid_constant__ Pa
     t0 += u0;
     t1 += u1;
   }
+  // warp s finishes channel s of the 32
   red[s][lane][0] = t0;
   red[s][lane][1] = t1;
   __syncthreads();
-  if (s == 0)
-    for (int r = 1; r < 32; ++r) t0 += red[r][lane][0], t1 += red[r][lane][1];
-  if (s != 0 || c >= P.C) return;
+  t0 = red[lane][s][0];
+  t1 = red[lane][s][1];
+#pragma unroll
+  for (int m = 16; m; m >>= 1) {
+    t0 += __shfl_xor_sync(0xffffffffu, t0, m);
+    t1 += __shfl_xor_sync(0xffffffffu, t1, m);
+  }
+  c = blockIdx.x * 32 + s;
+  if (lane != 0 || c >= P.C) return;
+  a = P.scale ? P.scale[c] : 1.f;
+  w = P.post_w ? P.post_w[c] : 1.f;
+  o = P.post_b ? P.post_b[c] : 0.f;
   if (pre) {
     if (P.dpre_w) P.dpre_w[c] = (float)t0;
     if (P.dpre_b) P.dpre_b[c] = (float)t1;
@@ -942,44 +1235,47 @@ static bool vectors_aligned(const Params& P) {
 }
 static int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
-template <typename IO, int CPT, int VEC, int MAXT>
+template <typename IO, int CPT, int VEC, bool ALONG, int MAXT, int MINB>
 static int cf_fwd(Params& P, cudaStream_t st) {
   const int S = ceil_div(P.C, CPT);
   P.tiles = ceil_div(P.HW, 32 * VEC);
-  const size_t smem = S > 1 ? (size_t)2 * S * 32 * VEC * sizeof(float2) : 0;
-  const int rc = allow_smem(cf_fwd_kernel<IO, CPT, VEC, MAXT>, smem);
+  const size_t smem = cf_smem(S, CPT, VEC, 4);
+  const int rc = allow_smem(cf_fwd_kernel<IO, CPT, VEC, ALONG, MAXT, MINB>, smem);
   if (rc != CVB_OK) return rc;
-  return launch_chained(cf_fwd_kernel<IO, CPT, VEC, MAXT>, dim3((unsigned)(P.tiles * P.B)), 32 * S, smem, st, P);
+  return launch_chained(cf_fwd_kernel<IO, CPT, VEC, ALONG, MAXT, MINB>, dim3((unsigned)(P.tiles * P.B)), 32 * S, smem, st, P);
 }
 template <typename IO>
 static int cf_fwd_any(Params& P, int sms, cudaStream_t st) {
-  // four pixels a thread where rows allow it and still give every SM two blocks; else one, which also takes odd rows
-  const bool four = P.HW % 4 == 0 && aligned(P, 4 * sizeof(IO)) && P.tokens >= (long long)2 * sms * 128;
-  if (P.C <= 128 && four) return cf_fwd<IO, 8, 4, 512>(P, st);
-  if (P.C <= 256) return cf_fwd<IO, 8, 1, 1024>(P, st);
-  if (P.C <= 1024) return cf_fwd<IO, 32, 1, 1024>(P, st);
+  // Four pixels a thread where that still gives half of the SMs a block, as vectors where rows allow it; else one.
+  const bool four = P.tokens >= (long long)64 * sms, along = P.HW % 4 == 0 && aligned(P, 4 * sizeof(IO));
+  if (P.C <= 64 && four) return along ? cf_fwd<IO, 8, 4, true, 256, 2>(P, st) : cf_fwd<IO, 8, 4, false, 256, 2>(P, st);
+  if (P.C <= 128 && four) return along ? cf_fwd<IO, 8, 4, true, 512, 1>(P, st) : cf_fwd<IO, 8, 4, false, 512, 1>(P, st);
+  if (P.C <= 256) return cf_fwd<IO, 8, 1, true, 1024, 1>(P, st);
+  if (P.C <= 1024) return cf_fwd<IO, 32, 1, true, 1024, 1>(P, st);
   P.tiles = ceil_div(P.HW, 32);
   return launch_chained(cf_fwd_wide_kernel<IO>, dim3((unsigned)(P.tiles * P.B)), 1024, 0, st, P);
 }
-template <typename IO, int NV, int V, int MAXT>
-static int cl_fwd(Params& P, cudaStream_t st) {
+template <typename IO, int NV, int V, int MAXT, int MINB>
+static int cl_fwd(Params& P, int sms, cudaStream_t st) {
   int tpr = 4;
   while (tpr * NV * V < P.C) tpr *= 2;
   const int threads = tpr > 256 ? tpr : 256;
   P.tpr = tpr;
-  return launch_chained(cl_fwd_kernel<IO, NV, V, MAXT>, dim3((unsigned)ceil_div(P.tokens, threads / tpr)), threads, 0, st, P);
+  const int blocks = ceil_div(P.tokens, threads / tpr);
+  return launch_chained(cl_fwd_kernel<IO, NV, V, MAXT, MINB>, dim3((unsigned)min(blocks, MINB * sms)), threads, 0, st, P);
 }
 template <typename IO>
-static int cl_fwd_any(Params& P, cudaStream_t st) {
+static int cl_fwd_any(Params& P, int sms, cudaStream_t st) {
   constexpr int V = 16 / (int)sizeof(IO);
   const bool vec = P.C % V == 0 && aligned(P, 16) && vectors_aligned(P);
-  if (P.C <= 2048) return vec ? cl_fwd<IO, 8 / V, V, 256>(P, st) : cl_fwd<IO, 8, 1, 256>(P, st);
-  return vec ? cl_fwd<IO, 16 / V, V, 1024>(P, st) : cl_fwd<IO, 16, 1, 1024>(P, st);
+  if (P.C <= 2048) return vec ? cl_fwd<IO, 8 / V, V, 256, sizeof(IO) == 4 ? 3 : 4>(P, sms, st) : cl_fwd<IO, 8, 1, 256, 3>(P, sms, st);
+  if (P.C <= 4096) return vec ? cl_fwd<IO, 8 / V, V, 512, 1>(P, sms, st) : cl_fwd<IO, 8, 1, 512, 1>(P, sms, st);
+  return vec ? cl_fwd<IO, 16 / V, V, 1024, 1>(P, sms, st) : cl_fwd<IO, 16, 1, 1024, 1>(P, sms, st);
 }
 
 int run_fwd(Params& P, int io, int sms, cudaStream_t st) {
   if (P.first) return io == CVB_F32 ? cf_fwd_any<float>(P, sms, st) : cf_fwd_any<__nv_bfloat16>(P, sms, st);
-  return io == CVB_F32 ? cl_fwd_any<float>(P, st) : cl_fwd_any<__nv_bfloat16>(P, st);
+  return io == CVB_F32 ? cl_fwd_any<float>(P, sms, st) : cl_fwd_any<__nv_bfloat16>(P, sms, st);
 }
 
 // Blocks of the backward kernel that add into sums of their own, for each image where the gate has a value for each image.
@@ -1001,13 +1297,23 @@ static int bwd_launch(K kernel, Params& P, int threads, size_t smem, long long u
   const dim3 grid((unsigned)(P.parts * (P.gate_kind == kGateImage ? P.B : 1)));
   return launch_chained(kernel, grid, threads, smem, st, P);
 }
-template <typename IO, int VEC, int MAXT, int MINB>
+template <typename IO, int VEC, bool ALONG, bool GATED, int MAXT, int MINB>
 static int cf_bwd(Params& P, int sms, cudaStream_t st) {
   const int S = ceil_div(P.C, 8);
   P.tiles = ceil_div(P.HW, 32 * VEC);
-  const int per_sm = MINB;
-  return bwd_launch(cf_bwd_kernel<IO, 8, VEC, MAXT, MINB>, P, 32 * S, S > 1 ? (size_t)2 * S * 32 * VEC * sizeof(float2) : 0, P.tiles,
-                    per_sm, sms, st);
+  using Px = Pixels<VEC, ALONG>;
+  const size_t slots = (size_t)S * ((GATED ? 5 : 4) * 8 * Px::template kSlot<IO> + 4 * Px::template kSlot<float>);
+  return bwd_launch(cf_bwd_kernel<IO, 8, VEC, ALONG, GATED, MAXT, MINB>, P, 32 * S, cf_smem(S, 8, VEC, 3) + slots, P.tiles, MINB, sms,
+                    st);
+}
+template <typename IO, bool GATED>
+static int cf_bwd_any(Params& P, int sms, cudaStream_t st) {
+  // as the forward: four pixels a thread (registers for 64 channels in a block of 256), or two
+  const bool four = P.tokens >= (long long)64 * sms, along4 = P.HW % 4 == 0 && aligned(P, 4 * sizeof(IO));
+  const bool along = P.HW % 2 == 0 && aligned(P, 2 * sizeof(IO));
+  if (P.C <= 64 && four) return along4 ? cf_bwd<IO, 4, true, GATED, 256, 1>(P, sms, st) : cf_bwd<IO, 4, false, GATED, 256, 1>(P, sms, st);
+  if (P.C <= 128) return along ? cf_bwd<IO, 2, true, GATED, 512, 1>(P, sms, st) : cf_bwd<IO, 2, false, GATED, 512, 1>(P, sms, st);
+  return cf_bwd<IO, 1, true, GATED, 1024, 1>(P, sms, st);
 }
 template <typename IO, int NV, int V, int MAXT, int MINB>
 static int cl_bwd(Params& P, int sms, cudaStream_t st) {
@@ -1017,23 +1323,21 @@ static int cl_bwd(Params& P, int sms, cudaStream_t st) {
   P.tpr = tpr;
   const long long per = P.gate_kind == kGateImage ? P.HW : P.tokens;
   const int slots = threads / (tpr > 32 ? tpr : 32);
-  return bwd_launch(cl_bwd_kernel<IO, NV, V, MAXT, MINB>, P, threads, slots > 1 ? (size_t)slots * 16 * P.C : 0,
+  const size_t joined = slots > 1 ? (size_t)slots * 16 * P.C : 0, ahead = cl_async<IO, NV, V>() ? (size_t)5 * NV * MAXT * V * sizeof(IO) : 0;
+  return bwd_launch(cl_bwd_kernel<IO, NV, V, MAXT, MINB>, P, threads, 64 * sizeof(float2) + (joined > ahead ? joined : ahead),
                     ceil_div(per, threads / tpr), MINB, sms, st);
 }
 template <typename IO>
 static int bwd_any(Params& P, int sms, cudaStream_t st) {
   if (P.first) {
-    if (P.C <= 64 && P.HW % 2 == 0 && aligned(P, 2 * sizeof(IO)) && P.tokens >= (long long)2 * sms * 64)
-      return cf_bwd<IO, 2, 256, 2>(P, sms, st);
-    if (P.C <= 64) return cf_bwd<IO, 1, 256, 3>(P, sms, st);
-    if (P.C <= 128) return cf_bwd<IO, 1, 512, 1>(P, sms, st);
-    if (P.C <= 256) return cf_bwd<IO, 1, 1024, 1>(P, sms, st);
+    if (P.C <= 256) return P.gate_kind == kGateFull ? cf_bwd_any<IO, true>(P, sms, st) : cf_bwd_any<IO, false>(P, sms, st);
     P.tiles = ceil_div(P.HW, 32);
     return bwd_launch(cf_bwd_wide_kernel<IO>, P, 1024, 32 * 32 * sizeof(float2) + (size_t)16 * P.C, P.tiles, 1, sms, st);
   }
   constexpr int V = 16 / (int)sizeof(IO);
   const bool vec = P.C % V == 0 && aligned(P, 16) && vectors_aligned(P);
   if (P.C <= 2048) return vec ? cl_bwd<IO, 8 / V, V, 256, 2>(P, sms, st) : cl_bwd<IO, 8, 1, 256, 2>(P, sms, st);
+  if (P.C <= 4096) return vec ? cl_bwd<IO, 8 / V, V, 512, 1>(P, sms, st) : cl_bwd<IO, 8, 1, 512, 1>(P, sms, st);
   return vec ? cl_bwd<IO, 16 / V, V, 1024, 1>(P, sms, st) : cl_bwd<IO, 16, 1, 1024, 1>(P, sms, st);
 }
 
