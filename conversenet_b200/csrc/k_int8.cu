@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(32 * kQuantWarps) quant_first_kernel(const __g
     for (int t = 0; t < S; ++t) a = largest(a, red[t][lane]);
   }
   if (!live) return;
-  const Quantiser q(a);
+  const Quantiser<sizeof(IO) == 2> q(a);
   if (s == 0) P.scale[token] = q.scale();
   for (int c0 = 32 * s; c0 < P.K; c0 += 32 * S) {
     if (P.K > 32 * S) {
@@ -74,71 +74,80 @@ __global__ void __launch_bounds__(32 * kQuantWarps) quant_first_kernel(const __g
   }
 }
 
-// channels_last: `tpr` threads a token, each with vectors of V channels; tokens of more than 16 tpr channels are read twice
+// channels_last: a warp a token, or fewer threads of it (tpr) where that is enough for a vector of V channels each; NV vectors of a
+// thread stay in registers as they were loaded.  Tokens of more than 32 NV V channels are read twice.  (With 256 threads a token
+// of 4096 channels most of the work was what a thread does once: 41 us for 8192 tokens.)
 template <typename IO, int V>
-__device__ __forceinline__ void load_vec(const void* p, long long i, float (&v)[V]) {
-  if constexpr (V == 1) {
-    v[0] = load1<IO>(p, i);
-  } else if constexpr (V == 4) {
-    const float4 a = *(const float4*)((const float*)p + i);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  } else {
-    const uint4 a = *(const uint4*)((const __nv_bfloat16*)p + i);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[2 * j] = __uint_as_float(w[j] << 16), v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+struct Raw;
+template <typename IO>
+struct Raw<IO, 1> {
+  float v;
+  __device__ __forceinline__ void load(const void* p, long long i) { v = load1<IO>(p, i); }
+  __device__ __forceinline__ void zero() { v = 0.f; }
+  __device__ __forceinline__ float top(float a) const { return largest(a, v); }
+};
+template <>
+struct Raw<float, 4> {
+  float4 v;
+  __device__ __forceinline__ void load(const void* p, long long i) { v = *(const float4*)((const float*)p + i); }
+  __device__ __forceinline__ void zero() { v = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ float top(float a) const { return largest(largest(a, v.x, v.y), v.z, v.w); }
+};
+template <>
+struct Raw<__nv_bfloat16, 8> {
+  uint4 v;
+  __device__ __forceinline__ void load(const void* p, long long i) { v = *(const uint4*)((const __nv_bfloat16*)p + i); }
+  __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ static float lo(uint32_t w) { return __uint_as_float(w << 16); }
+  __device__ __forceinline__ static float hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+  __device__ __forceinline__ float top(float a) const {
+    a = largest(largest(a, lo(v.x), hi(v.x)), lo(v.y), hi(v.y));
+    return largest(largest(a, lo(v.z), hi(v.z)), lo(v.w), hi(v.w));
   }
+};
+__device__ __forceinline__ void put(const Quantiser<false>& q, const Raw<float, 1>& r, signed char* to) { *to = (signed char)q.four(r.v, 0.f, 0.f, 0.f); }
+__device__ __forceinline__ void put(const Quantiser<true>& q, const Raw<__nv_bfloat16, 1>& r, signed char* to) { *to = (signed char)q.four(r.v, 0.f, 0.f, 0.f); }
+__device__ __forceinline__ void put(const Quantiser<false>& q, const Raw<float, 4>& r, signed char* to) {
+  *(uint32_t*)to = q.four(r.v.x, r.v.y, r.v.z, r.v.w);
 }
-template <typename IO, int V>
-__global__ void __launch_bounds__(1024) quant_last_kernel(const __grid_constant__ QuantParams P) {
+__device__ __forceinline__ void put(const Quantiser<true>& q, const Raw<__nv_bfloat16, 8>& r, signed char* to) {
+  using R = Raw<__nv_bfloat16, 8>;
+  *(uint2*)to = make_uint2(q.four(R::lo(r.v.x), R::hi(r.v.x), R::lo(r.v.y), R::hi(r.v.y)),
+                           q.four(R::lo(r.v.z), R::hi(r.v.z), R::lo(r.v.w), R::hi(r.v.w)));
+}
+
+template <typename IO, int V, int NV>
+__global__ void __launch_bounds__(256) quant_last_kernel(const __grid_constant__ QuantParams P) {
   pdl_start();
-  constexpr int NV = 16 / V;
-  __shared__ float red[32];
-  const int tpr = P.tpr, t = threadIdx.x & (tpr - 1), rows = blockDim.x / tpr;
-  const long long token = (long long)blockIdx.x * rows + threadIdx.x / tpr;
+  const int tpr = P.tpr, t = threadIdx.x & (tpr - 1), step = tpr * V;
+  const long long token = (long long)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
   const bool live = token < P.tokens;
-  const long long base = live ? token * P.K : 0;
-  float v[NV][V], a = 0.f;
-  for (int c0 = 0; c0 < P.K; c0 += 16 * tpr) {
+  const int K = live ? P.K : 0;
+  const IO* x = (const IO*)P.x + token * P.K;
+  Raw<IO, V> v[NV];
+  float a = 0.f;
+  for (int c0 = t * V; c0 < K; c0 += NV * step) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = c0 + (i * tpr + t) * V;
-      if (c < P.K) {
-        load_vec<IO, V>(P.x, base + c, v[i]);
-      } else {
+    for (int i = 0; i < NV; ++i)
+      if (c0 + i * step < K) v[i].load(x, c0 + i * step);
+      else v[i].zero();
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[i][j] = 0.f;
-      }
+    for (int i = 0; i < NV; ++i) a = v[i].top(a);
+  }
+  for (int o = tpr >> 1; o; o >>= 1) a = largest(a, __shfl_xor_sync(0xffffffffu, a, o));
+  if (!live) return;
+  const Quantiser<sizeof(IO) == 2> q(a);
+  if (t == 0) P.scale[token] = q.scale();
+  signed char* to = P.q + token * P.ldq;
+  for (int c0 = t * V; c0 < K; c0 += NV * step) {
+    if (K > NV * step) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (c0 + i * step < K) v[i].load(x, c0 + i * step);
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) a = largest(a, v[i][j]);
-  }
-  for (int o = (tpr < 32 ? tpr : 32) >> 1; o; o >>= 1) a = largest(a, __shfl_xor_sync(0xffffffffu, a, o));
-  if (tpr > 32) {
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
-    __syncthreads();
-    const int w0 = (threadIdx.x & ~(tpr - 1)) >> 5;
-    for (int j = 0; j < (tpr >> 5); ++j) a = largest(a, red[w0 + j]);
-  }
-  if (!live) return;
-  const Quantiser q(a);
-  if (t == 0) P.scale[token] = q.scale();
-  for (int c0 = 0; c0 < P.K; c0 += 16 * tpr) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = c0 + (i * tpr + t) * V;
-      if (c >= P.K) continue;
-      if (P.K > 16 * tpr) load_vec<IO, V>(P.x, base + c, v[i]);
-      signed char* to = P.q + token * P.ldq + c;
-      if constexpr (V == 1) {
-        *to = (signed char)q.four(v[i][0], 0.f, 0.f, 0.f);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; j += 4) *(uint32_t*)(to + j) = q.four(v[i][j], v[i][j + 1], v[i][j + 2], v[i][j + 3]);
-      }
-    }
+      if (c0 + i * step < K) put(q, v[i], to + c0 + i * step);
   }
 }
 
@@ -381,6 +390,16 @@ static int row_map(CUtensorMap* m, const signed char* p, long long rows, int K, 
              ? CVB_OK : CVB_ERR_BAD_ARGUMENT;
 }
 
+template <typename IO, int V>
+static int quantize_last(QuantParams& P, cudaStream_t st) {
+  P.tpr = 1;
+  while (P.tpr < 32 && P.tpr * V < P.K) P.tpr *= 2;
+  const dim3 grid((unsigned)ceil_div(P.tokens, 256 / P.tpr));
+  const int vectors = ceil_div(P.K, P.tpr * V);
+  if (vectors == 1) return launch_chained(quant_last_kernel<IO, V, 1>, grid, 256, 0, st, P);
+  if (vectors <= 4) return launch_chained(quant_last_kernel<IO, V, 4>, grid, 256, 0, st, P);
+  return launch_chained(quant_last_kernel<IO, V, 16>, grid, 256, 0, st, P);
+}
 template <typename IO>
 static int quantize(QuantParams& P, bool last, cudaStream_t st) {
   if (!last) {
@@ -389,12 +408,7 @@ static int quantize(QuantParams& P, bool last, cudaStream_t st) {
     return launch_chained(quant_first_kernel<IO>, dim3((unsigned)(P.tiles * P.B)), 32 * S, 0, st, P);
   }
   constexpr int V = 16 / (int)sizeof(IO);
-  P.tpr = 4;
-  while (P.tpr < 1024 && 16 * P.tpr < P.K) P.tpr *= 2;
-  const int threads = P.tpr > 256 ? P.tpr : 256;
-  const dim3 grid((unsigned)ceil_div(P.tokens, threads / P.tpr));
-  if (P.K % V == 0 && (size_t)P.x % 16 == 0) return launch_chained(quant_last_kernel<IO, V>, grid, threads, 0, st, P);
-  return launch_chained(quant_last_kernel<IO, 1>, grid, threads, 0, st, P);
+  return P.K % V == 0 && (size_t)P.x % 16 == 0 ? quantize_last<IO, V>(P, st) : quantize_last<IO, 1>(P, st);
 }
 
 template <typename IO, int NT>

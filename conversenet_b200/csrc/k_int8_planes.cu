@@ -1,5 +1,5 @@
-// 1x1 product in 8-bit integers over channels_first tensors, quantised on the way: out (B,N,HW) from x (B,K,HW), K up to 128
-// (fp32) or 256 (bf16).  Bound by the bytes of x and out, which are all it reads and writes beside the weights.
+// 1x1 product in 8-bit integers over channels_first tensors, quantised on the way: out (B,N,HW) from x (B,K,HW), K up to 128.
+// Bound by the bytes of x and out, which are all it reads and writes beside the weights.
 //
 // A pixel belongs to two threads from its loads to its stores, half of the channels each.  A group of 256 threads works on 128
 // pixels: the threads of a pixel find its largest magnitude, quantise their channels and write them to their lane of tensor memory,
@@ -65,42 +65,27 @@ __device__ __forceinline__ void plane_ld16(uint32_t t, int (&r)[16]) {
 __device__ __forceinline__ void plane_store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void plane_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// R registers of values of a pixel: R fp32 channels or 2 R bf16 ones
-template <typename IO, int R>
+// CH channels of a pixel, a register each, as they were loaded: nothing waits for them before they are used.  (bf16 values packed in
+// pairs were waited for at once, before the stores that should cover the loads: 1 x 128 -> 64 x 321 x 481 took 72 us.)
+template <typename IO, int CH>
 struct Values;
-template <int R>
-struct Values<float, R> {
-  static constexpr int kChannels = R;
-  uint32_t raw[R];
-  __device__ __forceinline__ void load(const float* p, long long HW, int n, bool live) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) raw[i] = live && i < n ? __float_as_uint(p[i * HW]) : 0u;
-  }
+template <int CH>
+struct Values<float, CH> {
+  uint32_t raw[CH];
+  __device__ __forceinline__ uint32_t at(const float* p) const { return __float_as_uint(*p); }
   __device__ __forceinline__ float operator[](int i) const { return __uint_as_float(raw[i]); }
 };
-template <int R>
-struct Values<__nv_bfloat16, R> {
-  static constexpr int kChannels = 2 * R;
-  uint32_t raw[R];
-  __device__ __forceinline__ void load(const __nv_bfloat16* p, long long HW, int n, bool live) {
-    const unsigned short* q = (const unsigned short*)p;
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const uint32_t lo = live && 2 * i < n ? q[2 * i * HW] : 0, hi = live && 2 * i + 1 < n ? q[(2 * i + 1) * HW] : 0;
-      raw[i] = lo | hi << 16;
-    }
-  }
-  __device__ __forceinline__ float operator[](int i) const {
-    return __uint_as_float(i & 1 ? raw[i >> 1] & 0xffff0000u : raw[i >> 1] << 16);
-  }
+template <int CH>
+struct Values<__nv_bfloat16, CH> {
+  uint32_t raw[CH];
+  __device__ __forceinline__ uint32_t at(const __nv_bfloat16* p) const { return *(const unsigned short*)p; }
+  __device__ __forceinline__ float operator[](int i) const { return __uint_as_float(raw[i] << 16); }
 };
 
-template <typename IO, int R>
+template <typename IO, int CH>
 __global__ void __launch_bounds__(kPlaneThreads* kPlaneGroups, 1) planes_kernel(const __grid_constant__ PlaneParams P) {
   // Before tensor memory is taken: a block of the kernel before, waiting for it, would wait for this one.
   pdl_start();
-  using V = Values<IO, R>;
-  constexpr int CH = V::kChannels;
   extern __shared__ __align__(16) unsigned char weights[];
   __shared__ float red[kPlaneGroups][2][kPlaneTile];
   __shared__ uint64_t bars[kPlaneGroups];
@@ -145,10 +130,18 @@ __global__ void __launch_bounds__(kPlaneThreads* kPlaneGroups, 1) planes_kernel(
 
   const long long step = (long long)gridDim.x * groups;
   long long tile = (long long)blockIdx.x * groups + g;
-  V v;
+  Values<IO, CH> v;
   auto fetch = [&](long long t) {
     const long long b = t / P.image_tiles, px = (t - b * P.image_tiles) * kPlaneTile + r;
-    v.load((const IO*)P.x + (b * P.K + half * CH) * P.HW + px, P.HW, P.K - half * CH, t < P.tiles && px < P.HW);
+    const IO* p = (const IO*)P.x + (b * P.K + half * CH) * P.HW + px;
+    const int n = t < P.tiles && px < P.HW ? P.K - half * CH : 0;
+    if (n >= CH) {
+#pragma unroll
+      for (int i = 0; i < CH; ++i, p += P.HW) v.raw[i] = v.at(p);
+    } else {
+#pragma unroll
+      for (int i = 0; i < CH; ++i, p += P.HW) v.raw[i] = i < n ? v.at(p) : 0u;
+    }
   };
   fetch(tile);
   for (; tile < P.tiles; tile += step) {
@@ -158,7 +151,7 @@ __global__ void __launch_bounds__(kPlaneThreads* kPlaneGroups, 1) planes_kernel(
     for (int i = 0; i < CH; i += 2) a = largest(a, v[i], v[i + 1]);
     red[g][half][r] = a;
     group_sync(g);
-    const Quantiser q(largest(a, red[g][half ^ 1][r]));
+    const Quantiser<sizeof(IO) == 2> q(largest(a, red[g][half ^ 1][r]));
     const float scale = q.scale();
 #pragma unroll
     for (int i = 0; i < CH / 16; ++i) {
@@ -189,10 +182,22 @@ __global__ void __launch_bounds__(kPlaneThreads* kPlaneGroups, 1) planes_kernel(
         int s[16];
         plane_ld16(lanes + c, s);
         tc::tmem_wait_ld();
+        IO* to = out + c * P.HW;
+        if (px >= P.HW) continue;
+        const int left = P.N - n0 - c;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const float y = fmaf((float)s[j] * scale, vec[n0 + c + j], vec[np + n0 + c + j]);
-          if (px < P.HW && n0 + c + j < P.N) plane_store(out + (c + j) * P.HW, y);
+        for (int j = 0; j < 16; j += 4) {
+          if (j >= left) break;
+          const float4 w = *(const float4*)(vec + n0 + c + j), o = *(const float4*)(vec + np + n0 + c + j);
+          const float ws[4] = {w.x, w.y, w.z, w.w}, os[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // the integer as fp32 (its magnitude is below 128 . 127 . 128 < 2^22) without the conversion unit
+            const float t = __int_as_float(s[j + i] + 0x4b400000) - 12582912.f;
+            const float y = fmaf(t * scale, ws[i], os[i]);
+            if (i == 0 || j + i < left) plane_store(to, y);
+            to += P.HW;
+          }
         }
       }
     }
@@ -206,20 +211,21 @@ __global__ void __launch_bounds__(kPlaneThreads* kPlaneGroups, 1) planes_kernel(
 
 static size_t plane_weight_bytes(int K, int N) { return (size_t)((K + 31) / 32 * 32) * ((N + 15) / 16 * 16); }
 
-// K that two threads hold in 64 registers each, weights that fit shared memory; few pixels with many output channels go to the
+// K that two threads hold in 64 registers each; weights that fit shared memory; few pixels with many output channels go to the
 // kernels that share the channels out to all multiprocessors
 bool planes_take(long long B, long long HW, int K, int N, int io, int sms) {
   const long long tiles = B * ((HW + kPlaneTile - 1) / kPlaneTile);
-  return K <= (io == CVB_F32 ? 128 : 256) && plane_weight_bytes(K, N) <= kPlaneWeights && (N <= 256 || tiles >= sms);
+  (void)io;
+  return K <= 128 && plane_weight_bytes(K, N) <= kPlaneWeights && (N <= 256 || tiles >= sms);
 }
 
-template <typename IO, int R>
+template <typename IO, int CH>
 static int launch(const PlaneParams& P, int sms, cudaStream_t st) {
   const size_t smem = plane_weight_bytes(P.K, P.N) + (size_t)(P.N + 15) / 16 * 16 * 8;
-  CVB_CUDA(cudaFuncSetAttribute(planes_kernel<IO, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+  CVB_CUDA(cudaFuncSetAttribute(planes_kernel<IO, CH>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
   const int groups = P.tiles > sms ? kPlaneGroups : 1;
   const long long blocks = (P.tiles + groups - 1) / groups;
-  return launch_chained(planes_kernel<IO, R>, dim3((unsigned)(blocks < sms ? blocks : sms)), kPlaneThreads * groups, smem, st, P);
+  return launch_chained(planes_kernel<IO, CH>, dim3((unsigned)(blocks < sms ? blocks : sms)), kPlaneThreads * groups, smem, st, P);
 }
 
 int run_planes(const void* x, const signed char* w, long long ldw, const float* w_scale, const float* bias, void* out, long long B,
@@ -229,7 +235,7 @@ int run_planes(const void* x, const signed char* w, long long ldw, const float* 
   P.image_tiles = (int)((HW + kPlaneTile - 1) / kPlaneTile);
   P.tiles = B * P.image_tiles;
   if (io == CVB_F32) return K <= 64 ? launch<float, 32>(P, sms, st) : launch<float, 64>(P, sms, st);
-  return K <= 128 ? launch<__nv_bfloat16, 32>(P, sms, st) : launch<__nv_bfloat16, 64>(P, sms, st);
+  return K <= 64 ? launch<__nv_bfloat16, 32>(P, sms, st) : launch<__nv_bfloat16, 64>(P, sms, st);
 }
 
 }  // namespace i8
