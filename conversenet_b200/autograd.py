@@ -253,28 +253,3 @@ class ConverseBlockFunction(torch.autograd.Function):
         gx, gcw, gcb, *gp = grads
         return (None, gx if need[1] else None, gcw if need[2] else None, gcb if need[3] else None, None, None,
                 *[q if n else None for q, n in zip(gp, need[6:])])
-
-
-class ResidualNormFunction(torch.autograd.Function):
-    """`functional.residual_norm` under autograd: the forward keeps the norms' means and spreads, the gradients come from one
-    pass over the tensors and one over partial sums (`csrc/k_seam.cu`).  `tensors`: x, branch, scale, gate, post_weight,
-    post_bias, pre_weight, pre_bias."""
-
-    @staticmethod
-    def forward(ctx, cfg, *tensors):
-        y, z, stats = _cabi.host().residual_norm(*tensors, *cfg, True)
-        ctx.cfg = cfg
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(stats, *tensors)
-        return y, z
-
-    @staticmethod
-    def backward(ctx, dy, dz):
-        return _residual_norm_backward(ctx, dy, dz)
-
-
-@once_differentiable
-def _residual_norm_backward(ctx, dy, dz):
-    stats, *tensors = ctx.saved_tensors
-    wanted = sum(1 << i for i, need in enumerate(ctx.needs_input_grad[1:]) if need)
-    return (None, *_cabi.host().residual_norm_backward(*tensors, *ctx.cfg, stats, dy, dz, wanted))

@@ -219,7 +219,7 @@ const char* cvb_strerror(int status) {
     case CVB_ERR_WORKSPACE: return "workspace missing or too small";
     case CVB_ERR_CUDA: return "CUDA runtime error (see cvb_last_cuda_error)";
     case CVB_ERR_KERNEL_TOO_LARGE: return "kernel_size larger than the padded plane";
-    case CVB_ERR_TOO_LARGE: return "plane too large for the fixed scratch array of this entry point";
+    case CVB_ERR_TOO_LARGE: return "size beyond a fixed maximum of this entry point (for planes: the scratch array)";
     default: return "unknown status";
   }
 }

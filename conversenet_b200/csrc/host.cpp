@@ -10,9 +10,12 @@
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <array>
 #include <cstdlib>
 #include <cstring>
 #include <memory>
@@ -620,7 +623,6 @@ PyMethodDef methods[] = {
     {"block_train", (PyCFunction)(void (*)(void))py_block_train, METH_FASTCALL, nullptr},
     {"block_backward", (PyCFunction)(void (*)(void))py_block_backward, METH_FASTCALL, nullptr},
     {"residual_norm", (PyCFunction)(void (*)(void))py_residual_norm, METH_FASTCALL, nullptr},
-    {"residual_norm_backward", (PyCFunction)(void (*)(void))py_residual_norm_backward, METH_FASTCALL, nullptr},
     {"quantize_tokens", (PyCFunction)(void (*)(void))py_quantize_tokens, METH_FASTCALL, nullptr},
     {"int8_product", (PyCFunction)(void (*)(void))py_int8_product, METH_FASTCALL, nullptr},
     {"pointwise_int8", (PyCFunction)(void (*)(void))py_pointwise_int8, METH_FASTCALL, nullptr},

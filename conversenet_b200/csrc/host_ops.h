@@ -17,167 +17,201 @@ void floating(const at::Tensor& t, const char* what) {
   if (t.defined() && !t.is_floating_point()) throw Failed(std::string(what) + " must be a floating-point tensor");
 }
 
-// The arguments that both directions of the seam share, checked
+// The residual seam's arguments, checked, and laid out for the kernels
+enum { kX, kBranch, kScale, kGate, kPostW, kPostB, kPreW, kPreB, kSeamTensors };
+struct SeamConfig {
+  double eps = 0;
+  bool rms = false, sigmoid = false, last = false;
+};
 struct Seam {
   cvb_residual_norm_args A;
-  at::Tensor x, branch, gate, vec[5];          // vec: scale, post_w, post_b, pre_w, pre_b as given
-  at::Tensor keep[5], gate_kept;               // as the kernels read them
+  std::array<at::Tensor, kSeamTensors> t;          // as given
+  at::Tensor x, branch, gate, vec[kSeamTensors];   // as the kernels read them
   bool empty = false;
 
-  // a: x-like, branch, scale, gate, post_w, post_b, pre_w, pre_b; eps, rms, sigmoid, channels_last
-  void read(const at::Tensor& like, PyObject* const* a) {
-    static const char* names[5] = {"scale", "post_weight", "post_bias", "pre_weight", "pre_bias"};
+  Seam(std::array<at::Tensor, kSeamTensors> given, const SeamConfig& c) : t(std::move(given)) {
+    static const char* names[] = {"x", "branch", "scale", "gate", "post_weight", "post_bias", "pre_weight", "pre_bias"};
     std::memset(&A, 0, sizeof(A));
-    x = like;
-    branch = optional(a[0], "branch");
-    vec[0] = optional(a[1], names[0]);
-    gate = optional(a[2], "gate");
-    for (int i = 1; i < 5; ++i) vec[i] = optional(a[2 + i], names[i]);
-    A.eps = (float)real(a[7]);
-    A.rms = PyObject_IsTrue(a[8]);
-    A.gate_act = PyObject_IsTrue(a[9]);
-    A.channels_last = PyObject_IsTrue(a[10]);
-    A.io_dtype = io_type(x);
-    if (A.channels_last ? x.dim() < 2 : x.dim() != 4)
-      throw Failed(A.channels_last ? "x must be (...,C) with at least one token dimension" : "x must be (B,C,H,W)");
+    A.eps = (float)c.eps; A.rms = c.rms; A.gate_act = c.sigmoid; A.channels_last = c.last;
+    const at::Tensor& x0 = t[kX];
+    A.io_dtype = io_type(x0);
+    if (c.last ? x0.dim() < 2 : x0.dim() != 4)
+      throw Failed(c.last ? "x must be (...,C) with at least one token dimension" : "x must be (B,C,H,W)");
     if (!(A.eps >= 0)) throw Failed("eps must not be negative");
-    const int64_t C = x.size(A.channels_last ? -1 : 1);
+    const int64_t C = x0.size(c.last ? -1 : 1);
     if (C < 1 || C > 16384) throw Failed("residual_norm takes 1 to 16384 channels, got " + std::to_string(C));
     A.C = (int)C;
-    same_device(branch, x, "branch");
-    if (branch.defined() && branch.sizes() != x.sizes()) throw Failed("branch must have the shape of x");
-    if (branch.defined() && branch.scalar_type() != x.scalar_type()) throw Failed("branch must have the type of x");
-    for (int i = 0; i < 5; ++i) {
-      same_device(vec[i], x, names[i]);
-      floating(vec[i], names[i]);
-      if (vec[i].defined() && vec[i].numel() != C) throw Failed(std::string(names[i]) + " must hold a value for each channel");
+    if (t[kBranch].sizes() != x0.sizes()) throw Failed("branch must have the shape of x");
+    if (t[kBranch].scalar_type() != x0.scalar_type()) throw Failed("branch must have the type of x");
+    for (int i = kBranch; i < kSeamTensors; ++i) {
+      if (!t[i].defined()) continue;
+      same_device(t[i], x0, names[i]);
+      floating(t[i], names[i]);
+      if (i != kBranch && i != kGate && t[i].numel() != C) throw Failed(std::string(names[i]) + " must hold a value for each channel");
     }
-    if ((vec[2].defined() && !vec[1].defined()) || (vec[4].defined() && !vec[3].defined()))
+    if ((t[kPostB].defined() && !t[kPostW].defined()) || (t[kPreB].defined() && !t[kPreW].defined()))
       throw Failed("a norm's bias needs its weight");
-    empty = x.numel() == 0;
+    empty = x0.numel() == 0;
     A.B = 1;
-    A.HW = empty ? 0 : x.numel() / C;
-    if (!A.channels_last) A.B = x.size(0), A.HW = x.size(2) * x.size(3);
-    if (!gate.defined()) return;
-    same_device(gate, x, "gate");
-    floating(gate, "gate");
-    if (gate.sizes() == x.sizes()) {
-      if (gate.scalar_type() != x.scalar_type()) throw Failed("a gate for each element must have the type of x");
+    A.HW = empty ? 0 : x0.numel() / C;
+    if (!c.last) A.B = x0.size(0), A.HW = x0.size(2) * x0.size(3);
+    const at::Tensor& g = t[kGate];
+    if (!g.defined()) return;
+    if (g.sizes() == x0.sizes()) {
+      if (g.scalar_type() != x0.scalar_type()) throw Failed("a gate for each element must have the type of x");
       A.gate_kind = CVB_GATE_FULL;
       return;
     }
-    bool image = gate.dim() == x.dim() && gate.size(0) == x.size(0);
-    for (int64_t d = 1; image && d < x.dim(); ++d)
-      image = gate.size(d) == (d == (A.channels_last ? x.dim() - 1 : 1) ? C : 1);
+    bool image = g.dim() == x0.dim() && g.size(0) == x0.size(0);
+    for (int64_t d = 1; image && d < x0.dim(); ++d) image = g.size(d) == (d == (c.last ? x0.dim() - 1 : 1) ? C : 1);
     if (!image) throw Failed("gate must have the shape of x, or hold a value for each image and channel");
     A.gate_kind = CVB_GATE_IMAGE;
-    if (A.channels_last && !empty) A.B = x.size(0), A.HW = x.numel() / C / A.B;
+    if (c.last && !empty) A.B = x0.size(0), A.HW = x0.numel() / C / A.B;
   }
-  // contiguous copies where they are needed (the interpreter's lock is not)
   void lay_out() {
-    if (branch.defined()) branch = branch.detach().contiguous();
-    A.branch = data<void>(branch);
-    const float* p[5];
-    for (int i = 0; i < 5; ++i) {
-      if (vec[i].defined()) keep[i] = f32(vec[i].detach());
-      p[i] = data<const float>(keep[i]);
-    }
-    A.scale = p[0]; A.post_w = p[1]; A.post_b = p[2]; A.pre_w = p[3]; A.pre_b = p[4];
-    if (A.gate_kind == CVB_GATE_FULL) gate_kept = gate.detach().contiguous();
-    if (A.gate_kind == CVB_GATE_IMAGE) gate_kept = f32(gate.detach());
-    A.gate = data<void>(gate_kept);
+    x = t[kX].detach().contiguous();
+    branch = t[kBranch].detach().contiguous();
+    A.x = x.data_ptr(); A.branch = branch.data_ptr();
+    for (int i = kScale; i < kSeamTensors; ++i)
+      if (t[i].defined() && i != kGate) vec[i] = f32(t[i].detach());
+    A.scale = data<const float>(vec[kScale]); A.post_w = data<const float>(vec[kPostW]); A.post_b = data<const float>(vec[kPostB]);
+    A.pre_w = data<const float>(vec[kPreW]); A.pre_b = data<const float>(vec[kPreB]);
+    if (A.gate_kind == CVB_GATE_FULL) gate = t[kGate].detach().contiguous();
+    if (A.gate_kind == CVB_GATE_IMAGE) gate = f32(t[kGate].detach());
+    A.gate = data<void>(gate);
+    A.stream = stream(x);
   }
 };
 
-// residual_norm(x, branch, scale, gate, post_w, post_b, pre_w, pre_b, eps, rms, sigmoid, channels_last, keep) ->
-// (y, z or None, stats or None)
+// y, z (undefined without pre_w), the means and spreads that the gradients need (undefined unless `keep`)
+std::array<at::Tensor, 3> seam_forward(Seam& s, bool keep) {
+  s.lay_out();
+  const auto opt = s.x.options().requires_grad(false);
+  at::Tensor y = at::empty(s.x.sizes(), opt), z, stats;
+  if (s.A.pre_w) z = at::empty(s.x.sizes(), opt);
+  if (keep && (s.A.pre_w || s.A.post_w)) stats = at::empty({4, s.A.B * s.A.HW}, opt.dtype(at::kFloat));
+  if (!s.empty) {
+    s.A.y = y.data_ptr(); s.A.z = data<void>(z); s.A.stats = data<float>(stats);
+    check(api.residual_norm_fwd(&s.A), "cvb_residual_norm_fwd");
+  }
+  return {y, z, stats};
+}
+
+// gradients of the tensors whose bit is set in `wanted`, from those of y and z (either may be undefined)
+std::array<at::Tensor, kSeamTensors> seam_backward(Seam& s, const at::Tensor& stats, at::Tensor dy, at::Tensor dz, unsigned wanted) {
+  std::array<at::Tensor, kSeamTensors> g;
+  s.lay_out();
+  const auto opt = s.x.options().requires_grad(false);
+  if (!s.A.pre_w) dz = at::Tensor();
+  for (int i = 0; i < kSeamTensors; ++i) {
+    const bool like_x = i == kX || i == kBranch || (i == kGate && s.A.gate_kind == CVB_GATE_FULL);
+    if ((wanted >> i & 1) && s.t[i].defined()) g[i] = at::empty(s.t[i].sizes(), like_x ? opt : opt.dtype(at::kFloat));
+  }
+  auto zero = [&](int from) {
+    for (int i = from; i < kSeamTensors; ++i)
+      if (g[i].defined()) g[i].zero_();
+  };
+  if (s.empty || (!dy.defined() && !dz.defined())) {
+    zero(0);
+  } else {
+    for (at::Tensor* t : {&dy, &dz}) {
+      if (t->defined()) *t = t->detach().to(s.x.scalar_type()).contiguous();
+      if (t->defined() && t->sizes() != s.x.sizes()) throw Failed("a gradient must have the shape of its output");
+    }
+    auto& A = s.A;
+    A.stats = data<float>(stats); A.dy = data<void>(dy); A.dz = data<void>(dz);
+    A.dx = data<void>(g[kX]); A.dbranch = data<void>(g[kBranch]); A.dscale = data<float>(g[kScale]); A.dgate = data<void>(g[kGate]);
+    A.dpost_w = data<float>(g[kPostW]); A.dpost_b = data<float>(g[kPostB]);
+    if (dz.defined()) A.dpre_w = data<float>(g[kPreW]), A.dpre_b = data<float>(g[kPreB]);
+    else zero(kPreW);
+    at::Tensor work;
+    if (A.dscale || A.dpost_w || A.dpost_b || A.dpre_w || A.dpre_b || (A.dgate && A.gate_kind == CVB_GATE_IMAGE)) {
+      A.workspace_bytes = api.residual_norm_workspace(A.C, A.B, A.gate_kind);
+      work = bytes_like(s.x, A.workspace_bytes);
+      A.workspace = work.data_ptr();
+    }
+    if (A.dx || A.dbranch || A.dgate || A.workspace) check(api.residual_norm_bwd(&A), "cvb_residual_norm_bwd");
+  }
+  for (int i = kScale; i < kSeamTensors; ++i)
+    if (g[i].defined() && g[i].scalar_type() != s.t[i].scalar_type()) g[i] = g[i].to(s.t[i].scalar_type());
+  return g;
+}
+
+// The seam under autograd, without the interpreter: a node of Python's took 140 us a step, of which the kernels are 30.
+struct SeamFunction : torch::autograd::Function<SeamFunction> {
+  using Opt = std::optional<at::Tensor>;
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& branch,
+                                                const Opt& scale, const Opt& gate, const Opt& post_w, const Opt& post_b,
+                                                const Opt& pre_w, const Opt& pre_b, SeamConfig c) {
+    auto in = [](const Opt& t) { return t.has_value() ? *t : at::Tensor(); };
+    Seam s({x, branch, in(scale), in(gate), in(post_w), in(post_b), in(pre_w), in(pre_b)}, c);
+    auto out = seam_forward(s, true);
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["eps"] = c.eps;
+    ctx->saved_data["flags"] = (int64_t)(c.rms | c.sigmoid << 1 | c.last << 2);
+    ctx->save_for_backward({out[2], s.t[0], s.t[1], s.t[2], s.t[3], s.t[4], s.t[5], s.t[6], s.t[7]});
+    if (out[1].defined()) return {out[0], out[1]};
+    return {out[0]};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    SeamConfig c;
+    c.eps = ctx->saved_data["eps"].toDouble();
+    const int64_t flags = ctx->saved_data["flags"].toInt();
+    c.rms = flags & 1; c.sigmoid = flags >> 1 & 1; c.last = flags >> 2 & 1;
+    const c10::cuda::CUDAGuard dev(saved[1].device());
+    std::array<at::Tensor, kSeamTensors> t;
+    unsigned wanted = 0;
+    size_t edge = 0;
+    for (int i = 0; i < kSeamTensors; ++i) {
+      t[i] = saved[1 + i];
+      if (t[i].defined() && ctx->needs_input_grad(edge++)) wanted |= 1u << i;
+    }
+    const bool again = at::GradMode::is_enabled();
+    const at::NoGradGuard no_grad;
+    Seam s(std::move(t), c);
+    auto g = seam_backward(s, saved[0], grads[0], grads.size() > 1 ? grads[1] : at::Tensor(), wanted);
+    torch::autograd::variable_list out(g.begin(), g.end());
+    if (again) {          // a graph of the backward is wanted: whoever goes through it learns that there is none
+      const at::AutoGradMode grad(true);
+      for (auto& o : out)
+        if (o.defined()) o.requires_grad_(true);
+      out = (*std::make_shared<torch::autograd::DelayedError>("residual_norm can be differentiated once", (int64_t)out.size()))(std::move(out));
+    }
+    out.emplace_back();
+    return out;
+  }
+};
+
+// residual_norm(x, branch, scale, gate, post_w, post_b, pre_w, pre_b, eps, rms, sigmoid, channels_last, under autograd) ->
+// (y, z or None)
 PyObject* py_residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     want(n, 13);
-    const at::Tensor& x0 = cuda_tensor(a[0], "x");
-    const c10::cuda::CUDAGuard dev(x0.device());
-    Seam s;
-    s.read(x0, a + 1);
-    if (!s.branch.defined()) throw Failed("branch must be a tensor");
-    const bool keep = PyObject_IsTrue(a[12]);
-    at::Tensor y, z, stats;
+    static const char* names[] = {"x", "branch", "scale", "gate", "post_weight", "post_bias", "pre_weight", "pre_bias"};
+    std::array<at::Tensor, kSeamTensors> t;
+    for (int i = 0; i < kSeamTensors; ++i) t[i] = i <= kBranch ? cuda_tensor(a[i], names[i]) : optional(a[i], names[i]);
+    SeamConfig c;
+    c.eps = real(a[8]);
+    c.rms = PyObject_IsTrue(a[9]); c.sigmoid = PyObject_IsTrue(a[10]); c.last = PyObject_IsTrue(a[11]);
+    const bool graph = PyObject_IsTrue(a[12]);
+    const c10::cuda::CUDAGuard dev(t[kX].device());
+    at::Tensor y, z;
     {
       const Unlocked unlocked;
-      s.lay_out();
-      const at::Tensor x = x0.detach().contiguous();
-      const auto opt = x.options().requires_grad(false);
-      y = at::empty(x.sizes(), opt);
-      if (s.A.pre_w) z = at::empty(x.sizes(), opt);
-      if (keep && (s.A.pre_w || s.A.post_w)) stats = at::empty({4, s.A.B * s.A.HW}, opt.dtype(at::kFloat));
-      if (!s.empty) {
-        s.A.x = x.data_ptr(); s.A.y = y.data_ptr(); s.A.z = data<void>(z); s.A.stats = data<float>(stats);
-        s.A.stream = stream(x);
-        check(api.residual_norm_fwd(&s.A), "cvb_residual_norm_fwd");
-      }
-    }
-    return Py_BuildValue("(NNN)", THPVariable_Wrap(std::move(y)), wrap_or_none(z), wrap_or_none(stats));
-  });
-}
-
-// residual_norm_backward(x, branch, scale, gate, post_w, post_b, pre_w, pre_b, eps, rms, sigmoid, channels_last, stats, dy or
-// None, dz or None, wanted) -> gradients of (x, branch, scale, gate, post_w, post_b, pre_w, pre_b), None where the bit of
-// `wanted` is not set
-PyObject* py_residual_norm_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded([&]() -> PyObject* {
-    want(n, 16);
-    const at::Tensor& x0 = cuda_tensor(a[0], "x");
-    const c10::cuda::CUDAGuard dev(x0.device());
-    Seam s;
-    s.read(x0, a + 1);
-    const at::Tensor stats = optional(a[12], "stats");
-    at::Tensor dy = optional(a[13], "dy"), dz = optional(a[14], "dz");
-    const long wanted = integer(a[15]);
-    at::Tensor g[8];
-    {
-      const Unlocked unlocked;
-      s.lay_out();
-      const auto opt = x0.options().requires_grad(false);
-      const at::Tensor* given[8] = {&x0, &s.branch, &s.vec[0], &s.gate, &s.vec[1], &s.vec[2], &s.vec[3], &s.vec[4]};
-      auto make = [&](int i, bool fp32) {
-        if ((wanted >> i & 1) && given[i]->defined())
-          g[i] = at::empty(given[i]->sizes(), fp32 ? opt.dtype(at::kFloat) : opt);
-      };
-      for (int i = 0; i < 8; ++i) make(i, i == 2 || i > 3 || (i == 3 && s.A.gate_kind == CVB_GATE_IMAGE));
-      if (s.empty || (!dy.defined() && !dz.defined())) {
-        for (auto& t : g)
-          if (t.defined()) t.zero_();
+      if (graph) {
+        auto opt = [&](int i) { return t[i].defined() ? SeamFunction::Opt(t[i]) : SeamFunction::Opt(); };
+        auto out = SeamFunction::apply(t[kX], t[kBranch], opt(kScale), opt(kGate), opt(kPostW), opt(kPostB), opt(kPreW), opt(kPreB), c);
+        y = out[0];
+        if (out.size() > 1) z = out[1];
       } else {
-        const at::Tensor x = x0.detach().contiguous();
-        auto like = [&](at::Tensor& t) {
-          if (t.defined()) t = t.detach().to(x.scalar_type()).contiguous();
-          if (t.defined() && t.sizes() != x.sizes()) throw Failed("a gradient must have the shape of its output");
-        };
-        like(dy);
-        like(dz);
-        auto& A = s.A;
-        A.x = x.data_ptr(); A.stats = data<float>(stats); A.dy = data<void>(dy); A.dz = data<void>(dz);
-        A.dx = data<void>(g[0]); A.dbranch = data<void>(g[1]); A.dscale = data<float>(g[2]); A.dgate = data<void>(g[3]);
-        A.dpost_w = data<float>(g[4]); A.dpost_b = data<float>(g[5]);
-        if (dz.defined()) {
-          A.dpre_w = data<float>(g[6]); A.dpre_b = data<float>(g[7]);
-        } else {
-          for (int i = 6; i < 8; ++i)
-            if (g[i].defined()) g[i].zero_();
-        }
-        at::Tensor work;
-        if (A.dscale || A.dpost_w || A.dpost_b || A.dpre_w || A.dpre_b || (A.dgate && A.gate_kind == CVB_GATE_IMAGE)) {
-          A.workspace_bytes = api.residual_norm_workspace(A.C, A.B, A.gate_kind);
-          work = bytes_like(x, A.workspace_bytes);
-          A.workspace = work.data_ptr();
-        }
-        A.stream = stream(x);
-        if (A.dx || A.dbranch || A.dgate || A.workspace) check(api.residual_norm_bwd(&A), "cvb_residual_norm_bwd");
+        Seam s(std::move(t), c);
+        auto out = seam_forward(s, false);
+        y = out[0];
+        z = out[1];
       }
-      for (int i = 2; i < 8; ++i)
-        if (g[i].defined() && g[i].scalar_type() != given[i]->scalar_type()) g[i] = g[i].to(given[i]->scalar_type());
     }
-    return Py_BuildValue("(NNNNNNNN)", wrap_or_none(g[0]), wrap_or_none(g[1]), wrap_or_none(g[2]), wrap_or_none(g[3]),
-                         wrap_or_none(g[4]), wrap_or_none(g[5]), wrap_or_none(g[6]), wrap_or_none(g[7]));
+    return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(y)), wrap_or_none(z));
   });
 }
 

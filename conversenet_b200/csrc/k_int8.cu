@@ -10,6 +10,7 @@
 #include <cuda.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "../../include/converse_b200.h"
 #include "cvb_int8.cuh"
@@ -235,7 +236,9 @@ struct Tile {
 __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-template <typename IO, int NT>
+// LAST: the rows of L are output channels, else pixels.  The sum is multiplied by the weights' scale first: a token's may be of any
+// size, and its product with a large sum no fp32 number although the result is one.
+template <typename IO, int NT, bool LAST>
 __global__ void __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ CUtensorMap mapL, const __grid_constant__ CUtensorMap mapR,
                const __grid_constant__ ProductParams P) {
@@ -334,13 +337,13 @@ product_kernel(const __grid_constant__ CUtensorMap mapL, const __grid_constant__
         const long long c = tile.col + c0;
         if (c >= P.cols) break;
         const float rs = c + lane < P.cols ? P.r_scale[c + lane] : 0.f;
-        const float rb = c + lane < P.cols && P.r_bias ? P.r_bias[c + lane] : 0.f;
+        const float rb = !LAST && c + lane < P.cols && P.r_bias ? P.r_bias[c + lane] : 0.f;
         int v[32];
         tmem_ld32i(tmem + acc * NT + c0 + ((uint32_t)(quadrant * 32) << 16), v);
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
-          const float s = __shfl_sync(0xffffffffu, rs, j), o = __shfl_sync(0xffffffffu, rb, j);
-          if (live && c + j < P.cols) store1(out + (c + j) * P.ldc, fmaf((float)v[j] * ls, s, o + lb));
+          const float s = __shfl_sync(0xffffffffu, rs, j), o = LAST ? 0.f : __shfl_sync(0xffffffffu, rb, j);
+          if (live && c + j < P.cols) store1(out + (c + j) * P.ldc, LAST ? fmaf((float)v[j] * ls, s, lb) : fmaf((float)v[j] * s, ls, o));
         }
       }
       tc::fence_before_sync();
@@ -411,7 +414,7 @@ static int quantize(QuantParams& P, bool last, cudaStream_t st) {
   return P.K % V == 0 && (size_t)P.x % 16 == 0 ? quantize_last<IO, V>(P, st) : quantize_last<IO, 1>(P, st);
 }
 
-template <typename IO, int NT>
+template <typename IO, int NT, bool LAST>
 static int product(ProductParams& P, const signed char* l, long long lrows, long long ldl, const signed char* r, long long rrows,
                    long long ldr, int sms, cudaStream_t st) {
   CUtensorMap mapL, mapR;
@@ -422,8 +425,8 @@ static int product(ProductParams& P, const signed char* l, long long lrows, long
   P.col_tiles = ceil_div(P.cols, NT);
   P.tiles = P.images * P.row_tiles * P.col_tiles;
   const size_t smem = (size_t)stages_of(NT) * stage_bytes(NT) + 1024;
-  CVB_CUDA(cudaFuncSetAttribute(product_kernel<IO, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  return launch_chained(product_kernel<IO, NT>, dim3((unsigned)(P.tiles < sms ? P.tiles : sms)), kThreads, smem, st, mapL, mapR, P);
+  CVB_CUDA(cudaFuncSetAttribute(product_kernel<IO, NT, LAST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  return launch_chained(product_kernel<IO, NT, LAST>, dim3((unsigned)(P.tiles < sms ? P.tiles : sms)), kThreads, smem, st, mapL, mapR, P);
 }
 template <typename IO>
 static int product_any(const signed char* q, long long ldq, const float* scale, const signed char* w, long long ldw,
@@ -444,9 +447,16 @@ static int product_any(const signed char* q, long long ldq, const float* scale, 
   const long long lrows = last ? N : tokens, rrows = last ? tokens : N, ldl = last ? ldw : ldq, ldr = last ? ldq : ldw;
   // the widest tile that leaves a tile for every multiprocessor
   auto tiles = [&](int NT) { return P.images * ceil_div(P.rows, kM) * ceil_div(P.cols, NT); };
-  if (P.cols > 128 && tiles(256) >= sms) return product<IO, 256>(P, l, lrows, ldl, r, rrows, ldr, sms, st);
-  if (P.cols > 64 && tiles(128) >= sms) return product<IO, 128>(P, l, lrows, ldl, r, rrows, ldr, sms, st);
-  return product<IO, 64>(P, l, lrows, ldl, r, rrows, ldr, sms, st);
+  const int NT = P.cols > 128 && tiles(256) >= sms ? 256 : P.cols > 64 && tiles(128) >= sms ? 128 : 64;
+  auto go = [&](auto nt, auto l_last) {
+    return product<IO, decltype(nt)::value, decltype(l_last)::value>(P, l, lrows, ldl, r, rrows, ldr, sms, st);
+  };
+  auto by_width = [&](auto l_last) {
+    return NT == 256   ? go(std::integral_constant<int, 256>(), l_last)
+           : NT == 128 ? go(std::integral_constant<int, 128>(), l_last)
+                       : go(std::integral_constant<int, 64>(), l_last);
+  };
+  return last ? by_width(std::true_type()) : by_width(std::false_type());
 }
 
 int run_quantize(const void* x, signed char* q, float* scale, long long B, long long HW, int K, long long ldq, bool last, int io,

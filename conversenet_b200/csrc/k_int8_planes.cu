@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kPlaneThreads* kPlaneGroups, 1) planes_kernel(
           for (int i = 0; i < 4; ++i) {
             // the integer as fp32 (its magnitude is below 128 . 127 . 128 < 2^22) without the conversion unit
             const float t = __int_as_float(s[j + i] + 0x4b400000) - 12582912.f;
-            const float y = fmaf(t * scale, ws[i], os[i]);
+            const float y = fmaf(t * ws[i], scale, os[i]);          // (tokens are of any size, weights of ordinary ones)
             if (i == 0 || j + i < left) plane_store(to, y);
             to += P.HW;
           }

@@ -920,18 +920,27 @@ __global__ void __launch_bounds__(MAXT, MINB) cl_fwd_kernel(const __grid_constan
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * tpr + t) * V;
-      float g[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) y[i][j] = fmaf((v[i][j] - mean) * rstd, wy[i][j], oy[i][j]);
       if (c < P.C && live) {
-        if (P.gate_kind) {
-          if (P.gate_kind == kGateFull) Vec<IO, V>::load(P.gate, base + c, g);
-          else cl_vector<V>((const float*)P.gate + token / P.HW * P.C, c, 0.f, g);
+        // (each way as the backward forms y again: where a token has one channel, y - mean has to be 0 there too)
+        float g[V];
+        if (P.gate_kind == kGateImage) {
+          cl_vector<V>((const float*)P.gate + token / P.HW * P.C, c, 0.f, g);
 #pragma unroll
-          for (int j = 0; j < V; ++j) y[i][j] *= gate_of(g[j], P.act);
+          for (int j = 0; j < V; ++j) {
+            g[j] = image_gate_of(g[j], P.act);
+            y[i][j] = fmaf((v[i][j] - mean) * rstd, wy[i][j] * g[j], oy[i][j] * g[j]) + x[i][j];
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < V; ++j) g[j] = 1.f;
+          if (P.gate_kind == kGateFull) {
+            Vec<IO, V>::load(P.gate, base + c, g);
+#pragma unroll
+            for (int j = 0; j < V; ++j) g[j] = gate_of(g[j], P.act);
+          }
+#pragma unroll
+          for (int j = 0; j < V; ++j) y[i][j] = fmaf(fmaf((v[i][j] - mean) * rstd, wy[i][j], oy[i][j]), g[j], x[i][j]);
         }
-#pragma unroll
-        for (int j = 0; j < V; ++j) y[i][j] += x[i][j];
         Vec<IO, V>::store(P.y, base + c, y[i]);
       } else {
 #pragma unroll

@@ -238,12 +238,8 @@ def residual_norm(x, branch, scale=None, gate=None, post_weight=None, post_bias=
     if gate_act not in (None, "sigmoid"):
         raise ValueError("gate_act must be None | 'sigmoid', got: %r" % (gate_act,))
     args = (branch, scale, gate, post_weight, post_bias, pre_weight, pre_bias)
-    cfg = (float(eps), norm == "rms", gate_act is not None, last)
-    if torch.is_grad_enabled() and (x.requires_grad or any(t is not None and t.requires_grad for t in args)):
-        from .autograd import ResidualNormFunction
-        y, z = ResidualNormFunction.apply(cfg, x, *args)
-    else:
-        y, z, _ = _cabi.host().residual_norm(x, *args, *cfg, False)
+    graph = torch.is_grad_enabled() and (x.requires_grad or any(t is not None and t.requires_grad for t in args))
+    y, z = _cabi.host().residual_norm(x, *args, float(eps), norm == "rms", gate_act is not None, last, graph)
     return y if pre_weight is None else (y, z)
 
 

@@ -331,3 +331,51 @@ class ConverseBlockAlphaVariant(ConverseBlock):
             x = self.alpha1 * self._branch1(x) + x
             x = self.alpha2 * self.conv2(x) + x
         return x
+
+
+class ResidualNorm(nn.Module):
+    """The seam between two branches of a block of any width (`functional.residual_norm`): y = x + scale * act(gate) *
+    N_post(branch) and z = N_pre(y).  `post`, `pre`, `scale`: with a norm of the branch, with a norm for the next branch, with
+    a learned scale for each channel (shaped and initialised as `ConverseBlockAlphaVariant`'s in channels_first).
+    `forward(x, branch, gate=None)` returns y, or (y, z) with `pre`."""
+
+    def __init__(self, channels, post=True, pre=True, scale=True, eps=1e-5, norm="layer", gate_act=None,
+                 data_format="channels_first"):
+        super().__init__()
+        self.channels, self.eps, self.norm, self.gate_act, self.data_format = channels, eps, norm, gate_act, data_format
+        for name, wanted in (("post", post), ("pre", pre)):
+            bias = wanted and norm == "layer"
+            self.register_parameter(name + "_weight", nn.Parameter(torch.ones(channels)) if wanted else None)
+            self.register_parameter(name + "_bias", nn.Parameter(torch.zeros(channels)) if bias else None)
+        shape = (1, channels, 1, 1) if data_format == "channels_first" else (channels,)
+        self.register_parameter("scale", nn.Parameter(torch.zeros(shape)) if scale else None)
+
+    def forward(self, x, branch, gate=None):
+        return CF.residual_norm(x, branch, self.scale, gate, self.post_weight, self.post_bias, self.pre_weight, self.pre_bias,
+                                self.eps, self.norm, self.gate_act if gate is not None else None, self.data_format)
+
+
+class Int8Pointwise(nn.Module):
+    """A 1x1 convolution or a linear layer in 8-bit integers, for inference (`functional.pointwise_int8`): weights as integers
+    with a scale for each output channel, every token of the input quantised by its largest channel."""
+
+    def __init__(self, layer):
+        super().__init__()
+        conv = isinstance(layer, nn.Conv2d)
+        if not conv and not isinstance(layer, nn.Linear):
+            raise TypeError("Int8Pointwise takes a 1x1 nn.Conv2d or an nn.Linear, got %s" % type(layer).__name__)
+        if conv and (layer.kernel_size != (1, 1) or layer.stride != (1, 1) or layer.padding not in ((0, 0), "valid") or
+                     layer.groups != 1):
+            raise ValueError("Int8Pointwise takes 1x1 convolutions of stride 1 without padding and groups")
+        self.data_format = "channels_first" if conv else "channels_last"
+        self.out_channels, self.in_channels = layer.weight.shape[:2]
+        q, scale = CF.quantize_weight(layer.weight)
+        # whole rows are kept, which begin at multiples of 16 bytes: a copy of the module on another device has them too
+        rows = torch.zeros(self.out_channels, (self.in_channels + 15) // 16 * 16, dtype=torch.int8, device=q.device)
+        rows[:, :self.in_channels] = q
+        self.register_buffer("weight_rows", rows)
+        self.register_buffer("weight_scale", scale)
+        self.register_buffer("bias", None if layer.bias is None else layer.bias.detach().float().clone())
+
+    def forward(self, x):
+        return CF.pointwise_int8(x, self.weight_rows[:, :self.in_channels], self.weight_scale, self.bias, self.data_format)
