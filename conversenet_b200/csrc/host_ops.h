@@ -216,21 +216,23 @@ PyObject* py_residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // ---- the norm of many tensors
-std::vector<at::Tensor> tensor_list(PyObject* o, const char* what) {
-  PyObject* fast = PySequence_Fast(o, "a sequence of tensors is wanted");
-  if (!fast) throw std::invalid_argument(what);
-  std::vector<at::Tensor> v;
-  const Py_ssize_t n = PySequence_Fast_GET_SIZE(fast);
-  v.reserve(n);
-  try {
-    for (Py_ssize_t i = 0; i < n; ++i) v.push_back(tensor(PySequence_Fast_GET_ITEM(fast, i), what));
-  } catch (...) {
-    Py_DECREF(fast);
-    throw;
+// A sequence of tensors, held as Python holds it for as long as this lives (a count of its own for each would take as long as the
+// rest of a call): only the interpreter's lock may be given up in between.
+struct TensorList {
+  PyObject* held = nullptr;
+  std::vector<const at::Tensor*> t;
+  TensorList() = default;
+  TensorList(const TensorList&) = delete;
+  ~TensorList() { Py_XDECREF(held); }
+  void read(PyObject* o, const char* what) {
+    held = PySequence_Tuple(o);
+    if (!held) throw std::invalid_argument(what);
+    const Py_ssize_t n = PyTuple_GET_SIZE(held);
+    t.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) t.push_back(&tensor(PyTuple_GET_ITEM(held, i), what));
   }
-  Py_DECREF(fast);
-  return v;
-}
+  size_t size() const { return t.size(); }
+};
 struct Range {
   uintptr_t from, to;
   bool operator<(const Range& o) const { return from < o.from; }
@@ -268,67 +270,77 @@ void refuse_overlap(const std::vector<cvb_span>& s) {
 PyObject* py_clip_by_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     want(n, 4);
-    std::vector<at::Tensor> in = tensor_list(a[0], "tensors"), out;
-    if (in.empty()) throw Failed("no tensors");
+    TensorList in, given;
+    in.read(a[0], "tensors");
+    if (!in.size()) throw Failed("no tensors");
     const bool scale = a[1] != Py_False, fresh = a[1] == Py_None, self = a[1] == Py_True;
     if (scale && !fresh && !self) {
-      out = tensor_list(a[1], "out");
-      if (out.size() != in.size()) throw Failed("out must hold a tensor for each of the tensors");
+      given.read(a[1], "out");
+      if (given.size() != in.size()) throw Failed("out must hold a tensor for each of the tensors");
     }
     const int kind = (int)integer(a[2]);
     const double max_norm = real(a[3]);
     if (scale && !(max_norm >= 0)) throw Failed("max_norm must not be negative");
-    for (const at::Tensor& t : in) {
-      if (!t.is_cuda()) throw Failed("the tensors must be CUDA tensors; this build has no CPU path");
-      if (t.layout() != at::kStrided) throw Failed("sparse tensors are not supported");
-      if (t.device() != in[0].device()) throw Failed("the tensors must be on one device");
-    }
-    const c10::cuda::CUDAGuard dev(in[0].device());
+    const at::Tensor& first = *in.t[0];
+    if (!first.is_cuda()) throw Failed("the tensors must be CUDA tensors; this build has no CPU path");
+    const c10::Device where = first.device();
+    const c10::cuda::CUDAGuard dev(where);
     at::Tensor norm;
+    std::vector<at::Tensor> made;          // new tensors
     {
       const Unlocked unlocked;
       std::vector<cvb_span> s(in.size());
-      if (fresh) out.reserve(in.size());
+      std::vector<at::Tensor> copies;      // of tensors that are read through one
+      if (fresh) made.reserve(in.size());
       for (size_t i = 0; i < in.size(); ++i) {
-        at::Tensor& t = in[i];
+        const at::Tensor& t = *in.t[i];
+        const void* from = nullptr;
+        auto copy = [&] {
+          copies.push_back(t.contiguous());
+          from = copies.back().const_data_ptr();
+        };
+        const c10::TensorImpl* impl = t.unsafeGetTensorImpl();
+        if (impl->layout() != at::kStrided) throw Failed("sparse tensors are not supported");
+        if (impl->device() != where) throw Failed("the tensors must be on one CUDA device; this build has no CPU path");
         s[i].in_type = s[i].out_type = io_type(t);
-        s[i].n = t.numel();
-        const bool flat = t.is_contiguous() || t.is_non_overlapping_and_dense();
-        if (fresh) out.push_back(at::empty_like(t, t.options().requires_grad(false),
+        s[i].n = impl->numel();
+        const bool whole = impl->is_contiguous(), flat = whole || t.is_non_overlapping_and_dense();
+        if (fresh) made.push_back(at::empty_like(t, t.options().requires_grad(false),
                                                 flat ? at::MemoryFormat::Preserve : at::MemoryFormat::Contiguous));
         if (self && !flat) throw Failed("a tensor to be scaled in place must fill its memory (no slices or expanded tensors)");
-        if (!out.empty()) {
-          const at::Tensor& o = out[i];
-          if (!o.is_cuda() || o.device() != t.device()) throw Failed("out must be on the device of the tensors");
-          if (o.layout() != at::kStrided || o.sizes() != t.sizes()) throw Failed("each tensor of out must have the shape of its tensor");
+        if (fresh || given.size()) {
+          const at::Tensor& o = fresh ? made[i] : *given.t[i];
+          const c10::TensorImpl* to = o.unsafeGetTensorImpl();
+          if (to->layout() != at::kStrided || to->sizes() != impl->sizes()) throw Failed("each tensor of out must have the shape of its tensor");
+          if (to->device() != where) throw Failed("out must be on the device of the tensors");
           s[i].out_type = io_type(o);
-          if (!(flat && o.strides() == t.strides())) {
-            if (!o.is_contiguous()) throw Failed("a tensor of out must be contiguous or have the strides of its tensor");
-            if (!t.is_contiguous()) t = t.contiguous();
+          if (!(whole && to->is_contiguous()) && !(flat && o.strides() == t.strides())) {
+            if (!to->is_contiguous()) throw Failed("a tensor of out must be contiguous or have the strides of its tensor");
+            if (!whole) copy();
           }
           s[i].out = o.data_ptr();
         } else if (!flat) {
-          t = t.contiguous();
+          copy();
         }
-        s[i].in = t.data_ptr();
+        s[i].in = from ? from : t.const_data_ptr();
         if (self) s[i].out = t.data_ptr();
       }
       if (scale) refuse_overlap(s);
-      norm = at::empty({}, in[0].options().dtype(at::kFloat).requires_grad(false));
+      norm = at::empty({}, first.options().dtype(at::kFloat).requires_grad(false));
       const size_t ws = api.clip_workspace((int)s.size());
-      at::Tensor work = bytes_like(in[0], ws);
+      at::Tensor work = bytes_like(first, ws);
       check(api.clip_by_norm(s.data(), (int)s.size(), kind, max_norm, scale, (float*)norm.data_ptr(), work.data_ptr(), ws,
-                             stream(in[0])),
+                             stream(first)),
             "cvb_clip_by_norm");
       // (autograd learns that they changed)
       if (scale && !fresh)
-        for (const at::Tensor& t : self ? in : out)
-          if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+        for (const at::Tensor* t : self ? in.t : given.t)
+          if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
     }
     if (!scale || self) return Py_BuildValue("(ON)", Py_None, THPVariable_Wrap(norm));
     if (!fresh) return Py_BuildValue("(ON)", a[1], THPVariable_Wrap(norm));
-    PyObject* list = PyList_New((Py_ssize_t)out.size());
-    for (size_t i = 0; i < out.size(); ++i) PyList_SET_ITEM(list, (Py_ssize_t)i, THPVariable_Wrap(out[i]));
+    PyObject* list = PyList_New((Py_ssize_t)made.size());
+    for (size_t i = 0; i < made.size(); ++i) PyList_SET_ITEM(list, (Py_ssize_t)i, THPVariable_Wrap(made[i]));
     return Py_BuildValue("(NN)", list, THPVariable_Wrap(norm));
   });
 }

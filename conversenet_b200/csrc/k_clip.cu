@@ -19,6 +19,7 @@ namespace cvb {
 constexpr int kClipThreads = 256, kClipPer = 32, kChunk = kClipThreads * kClipPer;   // elements of a chunk
 constexpr int kClipBlocksPerSm = 4;
 constexpr int kClipTensors = 960;          // of one launch
+constexpr unsigned kClipKept = 2300;       // chunks that the second kernel may find in the L2 cache
 
 struct ClipItem {
   const void* in;
@@ -26,7 +27,7 @@ struct ClipItem {
   unsigned first;          // its first chunk in the launch
   unsigned n_low;
   unsigned short n_high, types;      // elements: n_high . 2^32 + n_low; types: bit 0 in bf16, bit 1 out bf16, bit 2 vectors
-  unsigned pad;
+  unsigned ahead;          // elements that its first chunk lacks, so that the others begin at 16 bytes of in, or 128 of out
 };
 static_assert(sizeof(ClipItem) == 32, "");
 template <int N>
@@ -37,6 +38,7 @@ struct ClipParams {
   int partials;            // second kernel: how many
   int count;
   unsigned chunks;
+  unsigned passing;        // first kernel: chunks read as used for the last time
   int kind;                // 1, 2, or 0 for the largest magnitude
   int writes_norm;
   ClipItem item[N];
@@ -46,20 +48,27 @@ __device__ __forceinline__ float2 clip_bf2(unsigned v) {
   return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
 // eight elements from `i` on (all inside the tensor)
-template <bool BF16>
+template <bool BF16, bool LAST_USE>
 __device__ __forceinline__ void clip_load8(const void* p, long long i, float (&v)[8]) {
   if (BF16) {
-    const uint4 u = *(const uint4*)((const unsigned short*)p + i);
+    const uint4* q = (const uint4*)((const unsigned short*)p + i);
+    const uint4 u = LAST_USE ? __ldcs(q) : *q;
     const float2 a = clip_bf2(u.x), b = clip_bf2(u.y), c = clip_bf2(u.z), d = clip_bf2(u.w);
     v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y; v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
   } else {
-    const float4 a = *(const float4*)((const float*)p + i), b = *(const float4*)((const float*)p + i + 4);
+    const float4* q = (const float4*)((const float*)p + i);
+    const float4 a = LAST_USE ? __ldcs(q) : *q, b = LAST_USE ? __ldcs(q + 1) : q[1];
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   }
 }
-template <bool BF16>
+template <bool BF16, bool LAST_USE>
 __device__ __forceinline__ float clip_load1(const void* p, long long i) {
-  return BF16 ? __uint_as_float((unsigned)((const unsigned short*)p)[i] << 16) : ((const float*)p)[i];
+  if (BF16) {
+    const unsigned short* q = (const unsigned short*)p + i;
+    return __uint_as_float((unsigned)(LAST_USE ? __ldcs(q) : *q) << 16);
+  }
+  const float* q = (const float*)p + i;
+  return LAST_USE ? __ldcs(q) : *q;
 }
 
 // NaN stays
@@ -116,23 +125,20 @@ __device__ __forceinline__ int clip_find(const ClipParams<N>& P, unsigned chunk,
 // the elements of a chunk: [begin, end) of the tensor
 __device__ __forceinline__ void clip_range(const ClipItem& t, unsigned chunk, long long& begin, long long& end) {
   const long long n = ((long long)t.n_high << 32) + t.n_low;
-  begin = (long long)(chunk - t.first) * kChunk;
+  begin = (long long)(chunk - t.first) * kChunk - t.ahead;
   end = begin + kChunk < n ? begin + kChunk : n;
+  if (begin < 0) begin = 0;
 }
 
-template <bool BF16>
+template <bool BF16, bool LAST_USE>
 __device__ __forceinline__ void clip_chunk_norm(const ClipItem& t, long long begin, long long end, double& acc, int kind) {
   const int tid = threadIdx.x;
-  if (end - begin == kChunk && ((size_t)t.in & 15) == 0) {
+  if (end - begin == kChunk && ((size_t)((const char*)t.in + begin * (BF16 ? 2 : 4)) & 15) == 0) {
+    float v[kClipPer / 8][8];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float v[kClipPer / 16][8];
+    for (int j = 0; j < kClipPer / 8; ++j) clip_load8<BF16, LAST_USE>(t.in, begin + 8 * (j * kClipThreads + tid), v[j]);
 #pragma unroll
-      for (int j = 0; j < kClipPer / 16; ++j)
-        clip_load8<BF16>(t.in, begin + 8 * ((h * (kClipPer / 16) + j) * kClipThreads + tid), v[j]);
-#pragma unroll
-      for (int j = 0; j < kClipPer / 16; ++j) clip_add8(v[j], acc, kind);
-    }
+    for (int j = 0; j < kClipPer / 8; ++j) clip_add8(v[j], acc, kind);
     return;
   }
 #pragma unroll
@@ -141,7 +147,7 @@ __device__ __forceinline__ void clip_chunk_norm(const ClipItem& t, long long beg
     const long long at = begin + (long long)h * 8 * kClipThreads + tid;
     if (begin + (long long)h * 8 * kClipThreads >= end) break;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = at + j * kClipThreads < end ? clip_load1<BF16>(t.in, at + j * kClipThreads) : 0.f;
+    for (int j = 0; j < 8; ++j) v[j] = at + j * kClipThreads < end ? clip_load1<BF16, LAST_USE>(t.in, at + j * kClipThreads) : 0.f;
     clip_add8(v, acc, kind);
   }
 }
@@ -156,8 +162,14 @@ __global__ void __launch_bounds__(kClipThreads) clip_norm_kernel(const __grid_co
     const ClipItem& t = P.item[at];
     long long begin, end;
     clip_range(t, c, begin, end);
-    if (t.types & 1) clip_chunk_norm<true>(t, begin, end, acc, P.kind);
-    else clip_chunk_norm<false>(t, begin, end, acc, P.kind);
+    // what will not be in the L2 cache any more when the second kernel comes to it makes room for what will
+    if (c < P.passing) {
+      if (t.types & 1) clip_chunk_norm<true, true>(t, begin, end, acc, P.kind);
+      else clip_chunk_norm<false, true>(t, begin, end, acc, P.kind);
+    } else {
+      if (t.types & 1) clip_chunk_norm<true, false>(t, begin, end, acc, P.kind);
+      else clip_chunk_norm<false, false>(t, begin, end, acc, P.kind);
+    }
   }
   acc = clip_block_join(acc, P.kind);
   if (threadIdx.x == 0) P.partial[blockIdx.x] = acc;
@@ -167,42 +179,37 @@ template <bool INBF, bool OUTBF>
 __device__ __forceinline__ void clip_chunk_scale(const ClipItem& t, long long begin, long long end, float c) {
   const int tid = threadIdx.x;
   if (end - begin == kChunk && (t.types & 4)) {
+    float v[kClipPer / 8][8];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float v[kClipPer / 16][8];
+    for (int j = 0; j < kClipPer / 8; ++j) clip_load8<INBF, true>(t.in, begin + 8 * (j * kClipThreads + tid), v[j]);
 #pragma unroll
-      for (int j = 0; j < kClipPer / 16; ++j)
-        clip_load8<INBF>(t.in, begin + 8 * ((h * (kClipPer / 16) + j) * kClipThreads + tid), v[j]);
+    for (int j = 0; j < kClipPer / 8; ++j) {
+      const long long i = begin + 8 * (j * kClipThreads + tid);
+      if (OUTBF) {
+        __nv_bfloat162 w[4];
 #pragma unroll
-      for (int j = 0; j < kClipPer / 16; ++j) {
-        const long long i = begin + 8 * ((h * (kClipPer / 16) + j) * kClipThreads + tid);
-        if (OUTBF) {
-          __nv_bfloat162 w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = __floats2bfloat162_rn(v[j][2 * e] * c, v[j][2 * e + 1] * c);
-          *(uint4*)((__nv_bfloat16*)t.out + i) = *(const uint4*)w;
-        } else {
-          *(float4*)((float*)t.out + i) = make_float4(v[j][0] * c, v[j][1] * c, v[j][2] * c, v[j][3] * c);
-          *(float4*)((float*)t.out + i + 4) = make_float4(v[j][4] * c, v[j][5] * c, v[j][6] * c, v[j][7] * c);
-        }
+        for (int e = 0; e < 4; ++e) w[e] = __floats2bfloat162_rn(v[j][2 * e] * c, v[j][2 * e + 1] * c);
+        __stcs((uint4*)((__nv_bfloat16*)t.out + i), *(const uint4*)w);
+      } else {
+        __stcs((float4*)((float*)t.out + i), make_float4(v[j][0] * c, v[j][1] * c, v[j][2] * c, v[j][3] * c));
+        __stcs((float4*)((float*)t.out + i + 4), make_float4(v[j][4] * c, v[j][5] * c, v[j][6] * c, v[j][7] * c));
       }
     }
     return;
   }
+  // not both at vectors: neighbouring threads take neighbouring elements, all of them in flight at once; out's lines are whole
+  float v[kClipPer];
 #pragma unroll
-  for (int h = 0; h < kClipPer / 8; ++h) {
-    float v[8];
-    const long long at = begin + (long long)h * 8 * kClipThreads + tid;
-    if (begin + (long long)h * 8 * kClipThreads >= end) break;
+  for (int j = 0; j < kClipPer; ++j) {
+    const long long i = begin + j * kClipThreads + tid;
+    v[j] = i < end ? clip_load1<INBF, true>(t.in, i) : 0.f;
+  }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = at + j * kClipThreads < end ? clip_load1<INBF>(t.in, at + j * kClipThreads) : 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const long long i = at + j * kClipThreads;
-      if (i >= end) continue;
-      if (OUTBF) ((__nv_bfloat16*)t.out)[i] = __float2bfloat16_rn(v[j] * c);
-      else ((float*)t.out)[i] = v[j] * c;
-    }
+  for (int j = 0; j < kClipPer; ++j) {
+    const long long i = begin + j * kClipThreads + tid;
+    if (i >= end) continue;
+    if (OUTBF) ((__nv_bfloat16*)t.out)[i] = __float2bfloat16_rn(v[j] * c);
+    else ((float*)t.out)[i] = v[j] * c;
   }
 }
 
@@ -250,14 +257,18 @@ static int clip_launch(const cvb_span* spans, int from, int to, bool scale, cons
     const cvb_span& s = spans[i];
     if (s.n == 0) continue;
     ClipItem& t = P.item[count++];
-    t.in = s.in; t.out = s.out; t.first = chunks; t.pad = 0;
+    t.in = s.in; t.out = s.out; t.first = chunks;
+    const int in_size = s.in_type == CVB_BF16 ? 2 : 4, out_size = s.out_type == CVB_BF16 ? 2 : 4;
+    t.ahead = scale ? (unsigned)((size_t)s.out % 128 / out_size) : (unsigned)((size_t)s.in % 16 / in_size);
     t.n_low = (unsigned)s.n; t.n_high = (unsigned short)(s.n >> 32);
-    const bool vectors = ((size_t)s.in & 15) == 0 && ((size_t)s.out & 15) == 0;
+    const bool vectors = (((size_t)s.in - t.ahead * in_size) & 15) == 0 && (((size_t)s.out - t.ahead * out_size) & 15) == 0;
     t.types = (unsigned short)((s.in_type == CVB_BF16) | (s.out_type == CVB_BF16) << 1 | vectors << 2);
-    chunks += (unsigned)((s.n + kChunk - 1) / kChunk);
+    chunks += (unsigned)((s.n + t.ahead + kChunk - 1) / kChunk);
   }
   P.count = count;
   P.chunks = chunks;
+  // about what the L2 cache holds beside the outputs (2300 chunks of fp32 are 75 MB)
+  P.passing = chunks > kClipKept ? chunks - kClipKept : 0;
   blocks = clip_blocks(chunks, sms);
   if (!scale && !chunks) return CVB_OK;
   return launch_chained(scale ? clip_scale_kernel<N> : clip_norm_kernel<N>, dim3(blocks ? blocks : 1), kClipThreads, 0, st, P);
