@@ -19,6 +19,10 @@
 namespace cvb {
 namespace i8 {
 
+// the two halves of pdl_start (cvb_tma.cuh)
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // the larger magnitude of three; a NaN stays
 __device__ __forceinline__ float largest(float m, float a, float b) {
   float r;

@@ -248,8 +248,9 @@ product_kernel(const __grid_constant__ CUtensorMap mapL, const __grid_constant__
   __shared__ uint64_t full[ST], empty[ST], done[2], free_[2], drained;
   __shared__ uint32_t tmem_base;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // Before tensor memory is taken: a block of the kernel before, waiting for it, would wait for this one.
-  pdl_start();
+  // The wait comes before tensor memory is taken, and the next kernel is let in behind it: a block that held tensor memory while it
+  // waited for a kernel whose blocks still have to take theirs would wait for ever.
+  pdl_wait();
   if (threadIdx.x == 0) {
     for (int i = 0; i < ST; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&done[i], 1), mbar_init(&free_[i], kEpilogueWarps);
@@ -260,6 +261,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapL, const __grid_constant__
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
+  pdl_let_next();
   const uint32_t tmem = tmem_base;
   const int kblocks = (P.K + kBK - 1) / kBK;
   bool ok = true;

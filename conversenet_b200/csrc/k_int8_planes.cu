@@ -84,8 +84,9 @@ struct Values<__nv_bfloat16, CH> {
 
 template <typename IO, int CH>
 __global__ void __launch_bounds__(kPlaneThreads* kPlaneGroups, 1) planes_kernel(const __grid_constant__ PlaneParams P) {
-  // Before tensor memory is taken: a block of the kernel before, waiting for it, would wait for this one.
-  pdl_start();
+  // The wait comes before tensor memory is taken, and the next kernel is let in behind it: a block that held tensor memory while it
+  // waited for a kernel whose blocks still have to take theirs would wait for ever.
+  pdl_wait();
   extern __shared__ __align__(16) unsigned char weights[];
   __shared__ float red[kPlaneGroups][2][kPlaneTile];
   __shared__ uint64_t bars[kPlaneGroups];
@@ -123,6 +124,7 @@ __global__ void __launch_bounds__(kPlaneThreads* kPlaneGroups, 1) planes_kernel(
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
+  pdl_let_next();
   const uint32_t tmem = tmem_base + g * 256, lanes = tmem + ((uint32_t)(quadrant * 32) << 16);
   const uint32_t elected = tc::elect_one();
   uint32_t phase = 0;

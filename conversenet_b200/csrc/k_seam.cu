@@ -1255,10 +1255,14 @@ static int cf_fwd(Params& P, cudaStream_t st) {
 }
 template <typename IO>
 static int cf_fwd_any(Params& P, int sms, cudaStream_t st) {
-  // Four pixels a thread where that still gives half of the SMs a block, as vectors where rows allow it; else one.
-  const bool four = P.tokens >= (long long)64 * sms, along = P.HW % 4 == 0 && aligned(P, 4 * sizeof(IO));
-  if (P.C <= 64 && four) return along ? cf_fwd<IO, 8, 4, true, 256, 2>(P, st) : cf_fwd<IO, 8, 4, false, 256, 2>(P, st);
-  if (P.C <= 128 && four) return along ? cf_fwd<IO, 8, 4, true, 512, 1>(P, st) : cf_fwd<IO, 8, 4, false, 512, 1>(P, st);
+  // Several pixels a thread where that still gives half of the SMs a block, as vectors where rows allow it; else one.  Four of up
+  // to 64 channels (two blocks an SM).  Up to 96 two, with two blocks of 384 threads (4 x 96 x 65536 fp32: 79 us, four pixels 92);
+  // up to 128 four as vectors (118 us, two 114; bf16 102 and 107), two where they are 32 apart (bf16 120 us, four 161).
+  const bool several = P.tokens >= (long long)64 * sms;
+  const bool along2 = P.HW % 2 == 0 && aligned(P, 2 * sizeof(IO)), along4 = P.HW % 4 == 0 && aligned(P, 4 * sizeof(IO));
+  if (P.C <= 64 && several) return along4 ? cf_fwd<IO, 8, 4, true, 256, 2>(P, st) : cf_fwd<IO, 8, 4, false, 256, 2>(P, st);
+  if (P.C <= 96 && several) return along2 ? cf_fwd<IO, 8, 2, true, 384, 2>(P, st) : cf_fwd<IO, 8, 2, false, 384, 2>(P, st);
+  if (P.C <= 128 && several) return along4 ? cf_fwd<IO, 8, 4, true, 512, 1>(P, st) : cf_fwd<IO, 8, 2, false, 512, 2>(P, st);
   if (P.C <= 256) return cf_fwd<IO, 8, 1, true, 1024, 1>(P, st);
   if (P.C <= 1024) return cf_fwd<IO, 32, 1, true, 1024, 1>(P, st);
   P.tiles = ceil_div(P.HW, 32);
