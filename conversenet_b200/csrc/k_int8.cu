@@ -36,20 +36,31 @@ __device__ __forceinline__ float load1<float>(const void* p, long long i) { retu
 template <>
 __device__ __forceinline__ float load1<__nv_bfloat16>(const void* p, long long i) { return __bfloat162float(((const __nv_bfloat16*)p)[i]); }
 
-// channels_first: 32 pixels a block, warp s takes channels 32 s .. of each group of 32 S; more than one group is read twice
-constexpr int kQuantWarps = 8;
-template <typename IO>
-__global__ void __launch_bounds__(32 * kQuantWarps) quant_first_kernel(const __grid_constant__ QuantParams P) {
+// channels_first: 32 pixels a block, warp s takes channels 32 s .. of each group of 32 S; more than one group is read twice.  (Of
+// 4 x 3460 x 2550 bf16 with 8 warps a block the quantising took 260 us.)
+constexpr int kQuantWarps = 32;
+template <typename IO, int MAXT>
+__global__ void __launch_bounds__(MAXT) quant_first_kernel(const __grid_constant__ QuantParams P) {
   pdl_start();
   __shared__ float red[kQuantWarps][32];
   const int lane = threadIdx.x & 31, s = threadIdx.x >> 5, S = blockDim.x >> 5;
   const long long b = blockIdx.x / P.tiles, px = (long long)(blockIdx.x - b * P.tiles) * 32 + lane;
   const bool live = px < P.HW;
-  const long long base = b * P.K * P.HW + (live ? px : P.HW - 1), token = b * P.HW + px;
+  const IO* x = (const IO*)P.x + b * P.K * P.HW + (live ? px : P.HW - 1);
+  const long long token = b * P.HW + px;
   float v[32], a = 0.f;
-  for (int c0 = 32 * s; c0 < P.K; c0 += 32 * S) {
+  auto fetch = [&](int c0) {
+    const IO* p = x + c0 * P.HW;
+    if (c0 + 32 <= P.K) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = c0 + i < P.K ? load1<IO>(P.x, base + (c0 + i) * P.HW) : 0.f;
+      for (int i = 0; i < 32; ++i, p += P.HW) v[i] = load1<IO>(p, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i, p += P.HW) v[i] = c0 + i < P.K ? load1<IO>(p, 0) : 0.f;
+    }
+  };
+  for (int c0 = 32 * s; c0 < P.K; c0 += 32 * S) {
+    fetch(c0);
 #pragma unroll
     for (int i = 0; i < 32; i += 2) a = largest(a, v[i], v[i + 1]);
   }
@@ -62,93 +73,113 @@ __global__ void __launch_bounds__(32 * kQuantWarps) quant_first_kernel(const __g
   const Quantiser<sizeof(IO) == 2> q(a);
   if (s == 0) P.scale[token] = q.scale();
   for (int c0 = 32 * s; c0 < P.K; c0 += 32 * S) {
-    if (P.K > 32 * S) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = c0 + i < P.K ? load1<IO>(P.x, base + (c0 + i) * P.HW) : 0.f;
-    }
-    uint32_t w[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = q.four(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    if (P.K > 32 * S) fetch(c0);
     signed char* to = P.q + token * P.ldq + c0;
-    *(uint4*)to = make_uint4(w[0], w[1], w[2], w[3]);
-    if (c0 + 16 < P.K) *(uint4*)(to + 16) = make_uint4(w[4], w[5], w[6], w[7]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = q.four(v[16 * h + 4 * i], v[16 * h + 4 * i + 1], v[16 * h + 4 * i + 2], v[16 * h + 4 * i + 3]);
+      if (c0 + 16 * h < P.K) *(uint4*)(to + 16 * h) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
 }
 
-// channels_last: a warp a token, or fewer threads of it (tpr) where that is enough for a vector of V channels each; NV vectors of a
-// thread stay in registers as they were loaded.  Tokens of more than 32 NV V channels are read twice.  (With 256 threads a token
-// of 4096 channels most of the work was what a thread does once: 41 us for 8192 tokens.)
-template <typename IO, int V>
-struct Raw;
+// channels_last: a warp a token, or fewer threads of it (tpr) where that is enough for one piece each.  A row is read in the 16-byte
+// pieces of memory that it lies in, wherever it begins: the bytes that a piece gives belong `shift` places further to the left, so
+// a thread joins its own with its neighbour's before it stores them.  NV pieces of a thread stay in registers as they were loaded;
+// rows of more than 32 NV pieces are read twice.  (Element by element, rows of odd lengths took 228 us for 30456 x 1796 bf16.  With
+// 256 threads a token of 4096 channels most of the work was what a thread does once: 41 us for 8192 tokens.)
+__device__ __forceinline__ float half_lo(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float half_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+// the first or the last piece of a row, element by element (a function: it would be part of every load)
 template <typename IO>
-struct Raw<IO, 1> {
-  float v;
-  __device__ __forceinline__ void load(const void* p, long long i) { v = load1<IO>(p, i); }
-  __device__ __forceinline__ void zero() { v = 0.f; }
-  __device__ __forceinline__ float top(float a) const { return largest(a, v); }
-};
-template <>
-struct Raw<float, 4> {
-  float4 v;
-  __device__ __forceinline__ void load(const void* p, long long i) { v = *(const float4*)((const float*)p + i); }
-  __device__ __forceinline__ void zero() { v = make_float4(0.f, 0.f, 0.f, 0.f); }
-  __device__ __forceinline__ float top(float a) const { return largest(largest(a, v.x, v.y), v.z, v.w); }
-};
-template <>
-struct Raw<__nv_bfloat16, 8> {
+static __device__ __noinline__ uint4 edge_piece(const char* p, const char* from, const char* to) {
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 16 / (int)sizeof(IO); ++j) {
+    const char* q = p + j * (int)sizeof(IO);
+    if (q < from || q >= to) continue;
+    if (sizeof(IO) == 4) w[j & 3] = *(const uint32_t*)q;
+    else w[(j >> 1) & 3] |= (uint32_t)*(const unsigned short*)q << (16 * (j & 1));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename IO>
+struct Piece {
+  static constexpr int V = 16 / (int)sizeof(IO);
   uint4 v;
-  __device__ __forceinline__ void load(const void* p, long long i) { v = *(const uint4*)((const __nv_bfloat16*)p + i); }
-  __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ static float lo(uint32_t w) { return __uint_as_float(w << 16); }
-  __device__ __forceinline__ static float hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+  // the piece at `p`, of which [from, to) belongs to the row
+  __device__ __forceinline__ void load(const char* p, const char* from, const char* to) {
+    if (p >= from && p + 16 <= to) v = *(const uint4*)p;
+    else if (p + 16 <= from || p >= to) v = make_uint4(0, 0, 0, 0);
+    else v = edge_piece<IO>(p, from, to);
+  }
   __device__ __forceinline__ float top(float a) const {
-    a = largest(largest(a, lo(v.x), hi(v.x)), lo(v.y), hi(v.y));
-    return largest(largest(a, lo(v.z), hi(v.z)), lo(v.w), hi(v.w));
+    if (sizeof(IO) == 4)
+      return largest(largest(a, __uint_as_float(v.x), __uint_as_float(v.y)), __uint_as_float(v.z), __uint_as_float(v.w));
+    a = largest(largest(a, half_lo(v.x), half_hi(v.x)), half_lo(v.y), half_hi(v.y));
+    return largest(largest(a, half_lo(v.z), half_hi(v.z)), half_lo(v.w), half_hi(v.w));
+  }
+  // its V integers, the first one lowest
+  __device__ __forceinline__ uint64_t bytes(const Quantiser<sizeof(IO) == 2>& q) const {
+    if (sizeof(IO) == 4) return q.four(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+    const uint32_t lo = q.four(half_lo(v.x), half_hi(v.x), half_lo(v.y), half_hi(v.y));
+    const uint32_t hi = q.four(half_lo(v.z), half_hi(v.z), half_lo(v.w), half_hi(v.w));
+    return (uint64_t)hi << 32 | lo;
   }
 };
-__device__ __forceinline__ void put(const Quantiser<false>& q, const Raw<float, 1>& r, signed char* to) { *to = (signed char)q.four(r.v, 0.f, 0.f, 0.f); }
-__device__ __forceinline__ void put(const Quantiser<true>& q, const Raw<__nv_bfloat16, 1>& r, signed char* to) { *to = (signed char)q.four(r.v, 0.f, 0.f, 0.f); }
-__device__ __forceinline__ void put(const Quantiser<false>& q, const Raw<float, 4>& r, signed char* to) {
-  *(uint32_t*)to = q.four(r.v.x, r.v.y, r.v.z, r.v.w);
-}
-__device__ __forceinline__ void put(const Quantiser<true>& q, const Raw<__nv_bfloat16, 8>& r, signed char* to) {
-  using R = Raw<__nv_bfloat16, 8>;
-  *(uint2*)to = make_uint2(q.four(R::lo(r.v.x), R::hi(r.v.x), R::lo(r.v.y), R::hi(r.v.y)),
-                           q.four(R::lo(r.v.z), R::hi(r.v.z), R::lo(r.v.w), R::hi(r.v.w)));
-}
 
-template <typename IO, int V, int NV>
+template <typename IO, int NV>
 __global__ void __launch_bounds__(256) quant_last_kernel(const __grid_constant__ QuantParams P) {
   pdl_start();
-  const int tpr = P.tpr, t = threadIdx.x & (tpr - 1), step = tpr * V;
+  constexpr int V = Piece<IO>::V;
+  const int tpr = P.tpr, t = threadIdx.x & (tpr - 1);
   const long long token = (long long)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
   const bool live = token < P.tokens;
-  const int K = live ? P.K : 0;
-  const IO* x = (const IO*)P.x + token * P.K;
-  Raw<IO, V> v[NV];
-  float a = 0.f;
-  for (int c0 = t * V; c0 < K; c0 += NV * step) {
+  const char* all = (const char*)P.x;
+  const char *from = all + (live ? token : 0) * P.K * (long long)sizeof(IO), *to = live ? from + P.K * (long long)sizeof(IO) : from;
+  const int shift = (int)((size_t)from & 15) / (int)sizeof(IO);          // of the first piece's values lie before the row
+  const char* first = from - shift * (int)sizeof(IO);
+  const int pieces = (P.K + shift + V - 1) / V, rounds = (pieces + NV * tpr - 1) / (NV * tpr);
+  Piece<IO> v[NV];
+  auto fetch = [&](int round) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (c0 + i * step < K) v[i].load(x, c0 + i * step);
-      else v[i].zero();
+    for (int i = 0; i < NV; ++i) {
+      const char* p = first + ((long long)(round * NV + i) * tpr + t) * 16;
+      v[i].load(p, from, to);
+    }
+  };
+  float a = 0.f;
+  for (int r = 0; r < rounds; ++r) {
+    fetch(r);
 #pragma unroll
     for (int i = 0; i < NV; ++i) a = v[i].top(a);
   }
   for (int o = tpr >> 1; o; o >>= 1) a = largest(a, __shfl_xor_sync(0xffffffffu, a, o));
-  if (!live) return;
   const Quantiser<sizeof(IO) == 2> q(a);
-  if (t == 0) P.scale[token] = q.scale();
-  signed char* to = P.q + token * P.ldq;
-  for (int c0 = t * V; c0 < K; c0 += NV * step) {
-    if (K > NV * step) {
+  if (t == 0 && live) P.scale[token] = q.scale();
+  signed char* out = P.q + token * P.ldq;
+  // from the row's end to its beginning: `next` holds the bytes of the piece behind this thread's last one
+  uint64_t behind = 0;          // of the first piece of the tpr pieces behind
+  // (every lane of the warp takes part in the shuffles, with as many rounds as any of its rows)
+  int most = rounds;
+  for (int o = 16; o >= tpr; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+  for (int r = most - 1; r >= 0; --r) {
+    if (most > 1) fetch(r);
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (c0 + i * step < K) v[i].load(x, c0 + i * step);
+    for (int i = NV - 1; i >= 0; --i) {
+      const uint64_t own = v[i].bytes(q);
+      const uint64_t beside = __shfl_down_sync(0xffffffffu, own, 1, tpr), head = __shfl_sync(0xffffffffu, own, 0, tpr);
+      const uint64_t next = t == tpr - 1 ? behind : beside;
+      behind = head;
+      const int c = ((r * NV + i) * tpr + t) * V;
+      const uint64_t w = shift ? own >> (8 * shift) | next << (8 * (V - shift)) : own;
+      if (!live || c >= P.K) continue;
+      // (behind the last channel zeros: rows are that long)
+      if (V == 4) *(uint32_t*)(out + c) = (uint32_t)w;
+      else *(uint64_t*)(out + c) = w;
     }
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (c0 + i * step < K) put(q, v[i], to + c0 + i * step);
   }
 }
 
@@ -226,10 +257,10 @@ struct Tile {
   long long image;
   int row, col;          // first row of L in the image, first row of R
   __device__ __forceinline__ Tile(const ProductParams& P, long long t, int NT) {
-    const long long r = t / P.col_tiles;
-    col = (int)(t - r * P.col_tiles) * NT;
-    image = r / P.row_tiles;
-    row = (int)(r - image * P.row_tiles) * kM;
+    const unsigned r = (unsigned)t / (unsigned)P.col_tiles, b = r / (unsigned)P.row_tiles;
+    col = ((unsigned)t - r * P.col_tiles) * NT;
+    image = b;
+    row = (r - b * P.row_tiles) * kM;
   }
 };
 
@@ -247,6 +278,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapL, const __grid_constant__
   unsigned char* const ring = dynamic + (-smem_u32(dynamic) & 1023);       // the swizzle counts from 1024-byte boundaries
   __shared__ uint64_t full[ST], empty[ST], done[2], free_[2], drained;
   __shared__ uint32_t tmem_base;
+  __shared__ __align__(16) float columns[kEpilogueWarps][LAST ? NT / 2 : NT];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // The wait comes before tensor memory is taken, and the next kernel is let in behind it: a block that held tensor memory while it
   // waited for a kernel whose blocks still have to take theirs would wait for ever.
@@ -322,30 +354,51 @@ product_kernel(const __grid_constant__ CUtensorMap mapL, const __grid_constant__
     commit(&drained, elected);
     if (!warp_wait(&drained, 0)) ok = false;
   } else if (warp >= 4) {
-    // lane r of quadrant w & 3; the two warps of a quadrant take half of the columns each
+    // lane r of quadrant w & 3; the two warps of a quadrant take half of the columns each.  The columns' scales (and biases) lie in
+    // the warp's shared memory, loaded before the sums are waited for.
     const int quadrant = warp & 3, half = (warp - 4) >> 2;
+    float* const rs = columns[warp - 4];
+    float* const rb = rs + NT / 2;
     int acc = 0;
     uint32_t aph = 0;
     for (long long t = blockIdx.x; t < P.tiles; t += gridDim.x) {
       const Tile tile(P, t, NT);
-      const long long r = tile.row + quadrant * 32 + lane;
+      const int r = tile.row + quadrant * 32 + lane;
       const bool live = r < P.rows;
-      const float ls = live ? P.l_scale[tile.image * P.rows + r] : 0.f, lb = live && P.l_bias ? P.l_bias[r] : 0.f;
-      IO* out = (IO*)P.out + tile.image * P.image_stride + r;
+      const float ls = live ? P.l_scale[tile.image * P.rows + r] : 0.f, lb = LAST && live && P.l_bias ? P.l_bias[r] : 0.f;
+      const int c0 = tile.col + half * (NT / 2), left = (int)(P.cols - c0 < NT / 2 ? P.cols - c0 : NT / 2);
+      __syncwarp();          // the tile's before are read
+#pragma unroll
+      for (int c = 0; c < NT / 2; c += 32) {
+        const bool in = c + lane < left;
+        rs[c + lane] = in ? P.r_scale[c0 + c + lane] : 0.f;
+        if (!LAST) rb[c + lane] = in && P.r_bias ? P.r_bias[c0 + c + lane] : 0.f;
+      }
+      __syncwarp();
       ok = warp_wait(&done[acc], aph);
       if (!ok) break;
       tc::fence_after_sync();
-      for (int c0 = half * (NT / 2); c0 < (half + 1) * (NT / 2); c0 += 32) {
-        const long long c = tile.col + c0;
-        if (c >= P.cols) break;
-        const float rs = c + lane < P.cols ? P.r_scale[c + lane] : 0.f;
-        const float rb = !LAST && c + lane < P.cols && P.r_bias ? P.r_bias[c + lane] : 0.f;
-        int v[32];
-        tmem_ld32i(tmem + acc * NT + c0 + ((uint32_t)(quadrant * 32) << 16), v);
+      if (__any_sync(0xffffffffu, live)) {
+        IO* out = (IO*)P.out + tile.image * P.image_stride + (long long)c0 * P.ldc + r;
+        for (int c = 0; c < left; c += 32) {
+          int v[32];
+          tmem_ld32i(tmem + acc * NT + half * (NT / 2) + c + ((uint32_t)(quadrant * 32) << 16), v);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float s = __shfl_sync(0xffffffffu, rs, j), o = LAST ? 0.f : __shfl_sync(0xffffffffu, rb, j);
-          if (live && c + j < P.cols) store1(out + (c + j) * P.ldc, LAST ? fmaf((float)v[j] * ls, s, lb) : fmaf((float)v[j] * s, ls, o));
+          for (int j = 0; j < 32; j += 4) {
+            const float4 s4 = *(const float4*)(rs + c + j);
+            const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+            float o[4] = {lb, lb, lb, lb};
+            if (!LAST) {
+              const float4 o4 = *(const float4*)(rb + c + j);
+              o[0] = o4.x; o[1] = o4.y; o[2] = o4.z; o[3] = o4.w;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float y = LAST ? fmaf((float)v[j + i] * ls, s[i], o[i]) : fmaf((float)v[j + i] * s[i], ls, o[i]);
+              if (live && c + j + i < left) store1(out, y);
+              out += P.ldc;
+            }
+          }
         }
       }
       tc::fence_before_sync();
@@ -395,25 +448,29 @@ static int row_map(CUtensorMap* m, const signed char* p, long long rows, int K, 
              ? CVB_OK : CVB_ERR_BAD_ARGUMENT;
 }
 
-template <typename IO, int V>
+template <typename IO>
 static int quantize_last(QuantParams& P, cudaStream_t st) {
+  constexpr int V = Piece<IO>::V;
+  const bool even = P.K % V == 0 && (size_t)P.x % 16 == 0;          // every row begins with a piece
+  const int pieces = (P.K + (even ? 0 : V - 1) + V - 1) / V;
   P.tpr = 1;
-  while (P.tpr < 32 && P.tpr * V < P.K) P.tpr *= 2;
+  while (P.tpr < 32 && P.tpr < pieces) P.tpr *= 2;
   const dim3 grid((unsigned)ceil_div(P.tokens, 256 / P.tpr));
-  const int vectors = ceil_div(P.K, P.tpr * V);
-  if (vectors == 1) return launch_chained(quant_last_kernel<IO, V, 1>, grid, 256, 0, st, P);
-  if (vectors <= 4) return launch_chained(quant_last_kernel<IO, V, 4>, grid, 256, 0, st, P);
-  return launch_chained(quant_last_kernel<IO, V, 16>, grid, 256, 0, st, P);
+  const int each = ceil_div(pieces, P.tpr);
+  if (each == 1) return launch_chained(quant_last_kernel<IO, 1>, grid, 256, 0, st, P);
+  if (each <= 4) return launch_chained(quant_last_kernel<IO, 4>, grid, 256, 0, st, P);
+  return launch_chained(quant_last_kernel<IO, 16>, grid, 256, 0, st, P);
 }
 template <typename IO>
 static int quantize(QuantParams& P, bool last, cudaStream_t st) {
   if (!last) {
     P.tiles = ceil_div(P.HW, 32);
     const int S = min(kQuantWarps, ceil_div(P.K, 32));
-    return launch_chained(quant_first_kernel<IO>, dim3((unsigned)(P.tiles * P.B)), 32 * S, 0, st, P);
+    const dim3 grid((unsigned)(P.tiles * P.B));
+    return S <= 8 ? launch_chained(quant_first_kernel<IO, 256>, grid, 32 * S, 0, st, P)
+                  : launch_chained(quant_first_kernel<IO, 1024>, grid, 32 * S, 0, st, P);
   }
-  constexpr int V = 16 / (int)sizeof(IO);
-  return P.K % V == 0 && (size_t)P.x % 16 == 0 ? quantize_last<IO, V>(P, st) : quantize_last<IO, 1>(P, st);
+  return quantize_last<IO>(P, st);
 }
 
 template <typename IO, int NT, bool LAST>
@@ -426,6 +483,7 @@ static int product(ProductParams& P, const signed char* l, long long lrows, long
   P.row_tiles = ceil_div(P.rows, kM);
   P.col_tiles = ceil_div(P.cols, NT);
   P.tiles = P.images * P.row_tiles * P.col_tiles;
+  if (P.tiles > 0x7fffffffll) return CVB_ERR_TOO_LARGE;
   const size_t smem = (size_t)stages_of(NT) * stage_bytes(NT) + 1024;
   CVB_CUDA(cudaFuncSetAttribute(product_kernel<IO, NT, LAST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   return launch_chained(product_kernel<IO, NT, LAST>, dim3((unsigned)(P.tiles < sms ? P.tiles : sms)), kThreads, smem, st, mapL, mapR, P);

@@ -1277,13 +1277,25 @@ static int cl_fwd(Params& P, int sms, cudaStream_t st) {
   const int blocks = ceil_div(P.tokens, threads / tpr);
   return launch_chained(cl_fwd_kernel<IO, NV, V, MAXT, MINB>, dim3((unsigned)min(blocks, MINB * sms)), threads, 0, st, P);
 }
+// Elements that a thread reads and writes at once: 16 bytes, pairs, or single ones, as rows and addresses allow
+template <typename IO>
+static int cl_width(const Params& P) {
+  constexpr int V = 16 / (int)sizeof(IO);
+  if (P.C % V == 0 && aligned(P, 16) && vectors_aligned(P)) return V;
+  return P.C % 2 == 0 && aligned(P, 2 * sizeof(IO)) && vectors_aligned(P) ? 2 : 1;
+}
+template <typename IO, int V>
+static int cl_fwd_by_size(Params& P, int sms, cudaStream_t st) {
+  if (P.C <= 2048) return cl_fwd<IO, 8 / V, V, 256, sizeof(IO) == 2 && V == 8 ? 4 : 3>(P, sms, st);
+  if (P.C <= 4096) return cl_fwd<IO, 8 / V, V, 512, 1>(P, sms, st);
+  return cl_fwd<IO, 16 / V, V, 1024, 1>(P, sms, st);
+}
 template <typename IO>
 static int cl_fwd_any(Params& P, int sms, cudaStream_t st) {
-  constexpr int V = 16 / (int)sizeof(IO);
-  const bool vec = P.C % V == 0 && aligned(P, 16) && vectors_aligned(P);
-  if (P.C <= 2048) return vec ? cl_fwd<IO, 8 / V, V, 256, sizeof(IO) == 4 ? 3 : 4>(P, sms, st) : cl_fwd<IO, 8, 1, 256, 3>(P, sms, st);
-  if (P.C <= 4096) return vec ? cl_fwd<IO, 8 / V, V, 512, 1>(P, sms, st) : cl_fwd<IO, 8, 1, 512, 1>(P, sms, st);
-  return vec ? cl_fwd<IO, 16 / V, V, 1024, 1>(P, sms, st) : cl_fwd<IO, 16, 1, 1024, 1>(P, sms, st);
+  const int width = cl_width<IO>(P);
+  return width == 1 ? cl_fwd_by_size<IO, 1>(P, sms, st)
+         : width == 2 ? cl_fwd_by_size<IO, 2>(P, sms, st)
+                      : cl_fwd_by_size<IO, 16 / (int)sizeof(IO)>(P, sms, st);
 }
 
 int run_fwd(Params& P, int io, int sms, cudaStream_t st) {
@@ -1340,6 +1352,12 @@ static int cl_bwd(Params& P, int sms, cudaStream_t st) {
   return bwd_launch(cl_bwd_kernel<IO, NV, V, MAXT, MINB>, P, threads, 64 * sizeof(float2) + (joined > ahead ? joined : ahead),
                     ceil_div(per, threads / tpr), MINB, sms, st);
 }
+template <typename IO, int V>
+static int cl_bwd_by_size(Params& P, int sms, cudaStream_t st) {
+  if (P.C <= 2048) return cl_bwd<IO, 8 / V, V, 256, 2>(P, sms, st);
+  if (P.C <= 4096) return cl_bwd<IO, 8 / V, V, 512, 1>(P, sms, st);
+  return cl_bwd<IO, 16 / V, V, 1024, 1>(P, sms, st);
+}
 template <typename IO>
 static int bwd_any(Params& P, int sms, cudaStream_t st) {
   if (P.first) {
@@ -1347,11 +1365,10 @@ static int bwd_any(Params& P, int sms, cudaStream_t st) {
     P.tiles = ceil_div(P.HW, 32);
     return bwd_launch(cf_bwd_wide_kernel<IO>, P, 1024, 32 * 32 * sizeof(float2) + (size_t)16 * P.C, P.tiles, 1, sms, st);
   }
-  constexpr int V = 16 / (int)sizeof(IO);
-  const bool vec = P.C % V == 0 && aligned(P, 16) && vectors_aligned(P);
-  if (P.C <= 2048) return vec ? cl_bwd<IO, 8 / V, V, 256, 2>(P, sms, st) : cl_bwd<IO, 8, 1, 256, 2>(P, sms, st);
-  if (P.C <= 4096) return vec ? cl_bwd<IO, 8 / V, V, 512, 1>(P, sms, st) : cl_bwd<IO, 8, 1, 512, 1>(P, sms, st);
-  return vec ? cl_bwd<IO, 16 / V, V, 1024, 1>(P, sms, st) : cl_bwd<IO, 16, 1, 1024, 1>(P, sms, st);
+  const int width = cl_width<IO>(P);
+  return width == 1 ? cl_bwd_by_size<IO, 1>(P, sms, st)
+         : width == 2 ? cl_bwd_by_size<IO, 2>(P, sms, st)
+                      : cl_bwd_by_size<IO, 16 / (int)sizeof(IO)>(P, sms, st);
 }
 
 int run_bwd(Params& P, int io, int sms, cudaStream_t st) {

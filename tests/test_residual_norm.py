@@ -350,6 +350,52 @@ def test_streams_graphs_and_saved_tensors():
 
 
 @pytest.mark.gpu
+def test_saved_tensor_hooks_checkpointing_and_threads():
+    """What the backward reads passes through saved-tensor hooks; a checkpoint runs the forward again; calls from several threads on
+    streams of their own."""
+    import threading
+    from torch.utils.checkpoint import checkpoint
+    t = _case("first", 40, 2, 24, 28, torch.float32, "layer", True, "full", True)
+    names = [n for n in NAMES if n in t]
+    leaves = [t[n].requires_grad_(True) for n in names]
+    ref = torch.autograd.grad(_call(t, "first", "layer", True), leaves, (t["dy"], t["dz"]))
+    moved = []
+
+    def pack(v):
+        moved.append(v.shape)
+        return v.cpu()
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda v: v.cuda()):
+        out = _call(t, "first", "layer", True)
+    for a, b in zip(torch.autograd.grad(out, leaves, (t["dy"], t["dz"])), ref):
+        assert torch.equal(a, b)
+    assert len(moved) == len(names) + 1                        # the tensors, and the means and spreads
+    out = checkpoint(lambda x, b: _call(dict(t, x=x, branch=b), "first", "layer", True), t["x"], t["branch"], use_reentrant=False)
+    for a, b in zip(torch.autograd.grad(out, leaves, (t["dy"], t["dz"])), ref):
+        assert torch.equal(a, b)
+    wrong = []
+
+    def work(k):
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.default_stream())
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                with torch.no_grad():
+                    mine = {n: v.detach().clone() for n, v in t.items()}
+                ls = [mine[n].requires_grad_(True) for n in names]
+                got = torch.autograd.grad(_call(mine, "first", "layer", True), ls, (mine["dy"], mine["dz"]))
+                stream.synchronize()
+                wrong.extend(n for n, a, b in zip(names, got, ref) if not torch.equal(a, b))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong
+
+
+@pytest.mark.gpu
 def test_offsets_past_32_bits():
     """2^31 elements and more in a tensor: the last tokens against the formula."""
     HW = (1 << 27) + 64
