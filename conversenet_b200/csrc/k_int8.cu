@@ -108,13 +108,8 @@ static __device__ __noinline__ uint4 edge_piece(const char* p, const char* from,
 template <typename IO>
 struct Piece {
   static constexpr int V = 16 / (int)sizeof(IO);
+  using Bytes = std::conditional_t<V == 4, uint32_t, uint64_t>;
   uint4 v;
-  // the piece at `p`, of which [from, to) belongs to the row
-  __device__ __forceinline__ void load(const char* p, const char* from, const char* to) {
-    if (p >= from && p + 16 <= to) v = *(const uint4*)p;
-    else if (p + 16 <= from || p >= to) v = make_uint4(0, 0, 0, 0);
-    else v = edge_piece<IO>(p, from, to);
-  }
   __device__ __forceinline__ float top(float a) const {
     if (sizeof(IO) == 4)
       return largest(largest(a, __uint_as_float(v.x), __uint_as_float(v.y)), __uint_as_float(v.z), __uint_as_float(v.w));
@@ -122,32 +117,40 @@ struct Piece {
     return largest(largest(a, half_lo(v.z), half_hi(v.z)), half_lo(v.w), half_hi(v.w));
   }
   // its V integers, the first one lowest
-  __device__ __forceinline__ uint64_t bytes(const Quantiser<sizeof(IO) == 2>& q) const {
-    if (sizeof(IO) == 4) return q.four(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
-    const uint32_t lo = q.four(half_lo(v.x), half_hi(v.x), half_lo(v.y), half_hi(v.y));
-    const uint32_t hi = q.four(half_lo(v.z), half_hi(v.z), half_lo(v.w), half_hi(v.w));
-    return (uint64_t)hi << 32 | lo;
+  __device__ __forceinline__ Bytes bytes(const Quantiser<sizeof(IO) == 2>& q) const {
+    if constexpr (V == 4) {
+      return q.four(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z), __uint_as_float(v.w));
+    } else {
+      const uint32_t lo = q.four(half_lo(v.x), half_hi(v.x), half_lo(v.y), half_hi(v.y));
+      const uint32_t hi = q.four(half_lo(v.z), half_hi(v.z), half_lo(v.w), half_hi(v.w));
+      return (uint64_t)hi << 32 | lo;
+    }
   }
 };
 
-template <typename IO, int NV>
-__global__ void __launch_bounds__(256) quant_last_kernel(const __grid_constant__ QuantParams P) {
+// EVEN: every row begins with a piece and ends with one
+template <typename IO, int NV, bool EVEN>
+__global__ void __launch_bounds__(256, NV == 16 ? 2 : 3) quant_last_kernel(const __grid_constant__ QuantParams P) {
   pdl_start();
+  using Bytes = typename Piece<IO>::Bytes;
   constexpr int V = Piece<IO>::V;
   const int tpr = P.tpr, t = threadIdx.x & (tpr - 1);
   const long long token = (long long)blockIdx.x * (256 / tpr) + threadIdx.x / tpr;
   const bool live = token < P.tokens;
-  const char* all = (const char*)P.x;
-  const char *from = all + (live ? token : 0) * P.K * (long long)sizeof(IO), *to = live ? from + P.K * (long long)sizeof(IO) : from;
-  const int shift = (int)((size_t)from & 15) / (int)sizeof(IO);          // of the first piece's values lie before the row
-  const char* first = from - shift * (int)sizeof(IO);
-  const int pieces = (P.K + shift + V - 1) / V, rounds = (pieces + NV * tpr - 1) / (NV * tpr);
+  const int K = live ? P.K : 0;
+  const IO* row = (const IO*)P.x + (live ? token : 0) * P.K;
+  const int shift = EVEN ? 0 : (int)((size_t)row & 15) / (int)sizeof(IO);          // values of the first piece that lie before the row
+  const char* first = (const char*)(row - shift);
+  const int pieces = (K + shift + V - 1) / V, whole_from = shift != 0, whole_to = (K + shift) / V;
+  const int rounds = (pieces + NV * tpr - 1) / (NV * tpr);
   Piece<IO> v[NV];
   auto fetch = [&](int round) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const char* p = first + ((long long)(round * NV + i) * tpr + t) * 16;
-      v[i].load(p, from, to);
+      const int p = (round * NV + i) * tpr + t;
+      if (p >= whole_from && p < whole_to) v[i].v = *(const uint4*)(first + (long long)p * 16);
+      else if (EVEN || p >= pieces) v[i].v = make_uint4(0, 0, 0, 0);
+      else v[i].v = edge_piece<IO>(first + (long long)p * 16, (const char*)row, (const char*)(row + K));
     }
   };
   float a = 0.f;
@@ -160,25 +163,23 @@ __global__ void __launch_bounds__(256) quant_last_kernel(const __grid_constant__
   const Quantiser<sizeof(IO) == 2> q(a);
   if (t == 0 && live) P.scale[token] = q.scale();
   signed char* out = P.q + token * P.ldq;
-  // from the row's end to its beginning: `next` holds the bytes of the piece behind this thread's last one
-  uint64_t behind = 0;          // of the first piece of the tpr pieces behind
-  // (every lane of the warp takes part in the shuffles, with as many rounds as any of its rows)
+  // Every lane of the warp takes part in the shuffles, with as many rounds as any of its rows; from the rows' ends to their
+  // beginnings, for the bytes behind a thread's own are needed first.
   int most = rounds;
   for (int o = 16; o >= tpr; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+  Bytes behind = 0;          // of the first of the tpr pieces behind
   for (int r = most - 1; r >= 0; --r) {
     if (most > 1) fetch(r);
 #pragma unroll
     for (int i = NV - 1; i >= 0; --i) {
-      const uint64_t own = v[i].bytes(q);
-      const uint64_t beside = __shfl_down_sync(0xffffffffu, own, 1, tpr), head = __shfl_sync(0xffffffffu, own, 0, tpr);
-      const uint64_t next = t == tpr - 1 ? behind : beside;
-      behind = head;
+      Bytes w = v[i].bytes(q);
+      if (!EVEN) {
+        const Bytes own = w, beside = __shfl_down_sync(0xffffffffu, own, 1, tpr), next = t == tpr - 1 ? behind : beside;
+        if (NV > 1 || most > 1) behind = __shfl_sync(0xffffffffu, own, 0, tpr);
+        if (shift) w = own >> (8 * shift) | next << (8 * (V - shift));
+      }
       const int c = ((r * NV + i) * tpr + t) * V;
-      const uint64_t w = shift ? own >> (8 * shift) | next << (8 * (V - shift)) : own;
-      if (!live || c >= P.K) continue;
-      // (behind the last channel zeros: rows are that long)
-      if (V == 4) *(uint32_t*)(out + c) = (uint32_t)w;
-      else *(uint64_t*)(out + c) = w;
+      if (c < K) *(Bytes*)(out + c) = w;          // (behind the last channel zeros: rows are that long)
     }
   }
 }
@@ -457,9 +458,14 @@ static int quantize_last(QuantParams& P, cudaStream_t st) {
   while (P.tpr < 32 && P.tpr < pieces) P.tpr *= 2;
   const dim3 grid((unsigned)ceil_div(P.tokens, 256 / P.tpr));
   const int each = ceil_div(pieces, P.tpr);
-  if (each == 1) return launch_chained(quant_last_kernel<IO, 1>, grid, 256, 0, st, P);
-  if (each <= 4) return launch_chained(quant_last_kernel<IO, 4>, grid, 256, 0, st, P);
-  return launch_chained(quant_last_kernel<IO, 16>, grid, 256, 0, st, P);
+  auto go = [&](auto nv) {
+    constexpr int NV = decltype(nv)::value;
+    return even ? launch_chained(quant_last_kernel<IO, NV, true>, grid, 256, 0, st, P)
+                : launch_chained(quant_last_kernel<IO, NV, false>, grid, 256, 0, st, P);
+  };
+  return each == 1   ? go(std::integral_constant<int, 1>())
+         : each <= 4 ? go(std::integral_constant<int, 4>())
+                     : go(std::integral_constant<int, 16>());
 }
 template <typename IO>
 static int quantize(QuantParams& P, bool last, cudaStream_t st) {
