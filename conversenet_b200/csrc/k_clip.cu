@@ -16,10 +16,10 @@
 
 namespace cvb {
 
-constexpr int kClipThreads = 256, kClipPer = 32, kChunk = kClipThreads * kClipPer;   // elements of a chunk
-constexpr int kClipBlocksPerSm = 4;
+constexpr int kClipThreads = 256, kClipPer = 16, kChunk = kClipThreads * kClipPer;   // elements of a chunk
+constexpr int kClipBlocksPerSm = 8;
 constexpr int kClipTensors = 960;          // of one launch
-constexpr unsigned kClipKept = 2300;       // chunks that the second kernel may find in the L2 cache
+constexpr unsigned kClipKept = 4600;       // chunks that the second kernel may find in the L2 cache
 
 struct ClipItem {
   const void* in;
@@ -267,7 +267,7 @@ static int clip_launch(const cvb_span* spans, int from, int to, bool scale, cons
   }
   P.count = count;
   P.chunks = chunks;
-  // about what the L2 cache holds beside the outputs (2300 chunks of fp32 are 75 MB)
+  // about what the L2 cache holds beside the outputs (4600 chunks of fp32 are 75 MB)
   P.passing = chunks > kClipKept ? chunks - kClipKept : 0;
   blocks = clip_blocks(chunks, sms);
   if (!scale && !chunks) return CVB_OK;
