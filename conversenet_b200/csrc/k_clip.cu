@@ -11,6 +11,10 @@
 // Squares of fp32 numbers leave fp32's range (1e20 squared).  A thread adds the squares of eight elements in fp32 where their
 // largest magnitude lies between 2^-40 and 2^50 (what is then lost to underflow is below 2^-60 of the sum), else it squares
 // them in 64 bits; each sum of eight goes into a 64-bit one.
+//
+// 48 tensors, 64 M fp32 values, outputs at odd places: 43 us for the norm, 138 for both (78 if every value were read once; the norm has
+// to be known before the first store).  The scaling kernel goes backwards, from what is still in the L2 cache; outputs are stored from
+// 128-byte boundaries on (from anywhere: 150 us).  284 tensors, 0.56 M values: 13 us on the device.
 #include "../../include/converse_b200.h"
 #include "cvb_internal.h"
 

@@ -7,6 +7,10 @@
 // last K and the last row.  One block a multiprocessor walks over tiles of 128 x NT: a warp that copies, a warp that issues the
 // MMAs, eight warps that scale and store; two accumulators, so that a tile is stored while the next one is computed.
 // Every wait is bounded; a role that gives up sets the status word and ends, and the others follow.
+//
+// What bounds it: the tensor pipe where K is long (8192 x 4096 -> 4096: 91 us, the pipe active 80 % of the cycles, 3.0 POP/s);
+// bytes and the epilogue's conversions and stores where it is short (192360 x 117 -> 16 fp32: 21 us; 55 with the columns' scales
+// passed by shuffles and an address multiplied out for every store).
 #include <cuda.h>
 
 #include <atomic>

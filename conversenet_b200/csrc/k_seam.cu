@@ -16,6 +16,11 @@
 // meet by shuffles, and through shared memory where a token has more than a warp.  Backward: blocks walk over tokens with the
 // four sums of their channels in registers and leave one partial result each; a second kernel adds them in order, in 64 bits.
 // Means, spreads and sums are held in 32 bits or more; z comes from y before y is rounded to the tensors' type.
+//
+// 8 x 64 x 256 x 256 fp32 with both norms: forward 89 us (82 at the measured copy rate), gradients 134 (123).  On the way: 145 us with
+// every thread adding up all warps' sums and vectors read from global memory (120 instructions an element); gradients 280 us with a
+// tile's loads waited for at its beginning, 194 with two pixels a thread instead of four.  bf16 tokens with a gate (65472 x 1024): 211 us
+// (102), gradients 281 (164), bound by instructions: conversions, the gate's exponential and two norms' sums of 8 values a thread.
 #include "../../include/converse_b200.h"
 #include "cvb_internal.h"
 #include "cvb_seam.h"

@@ -357,7 +357,8 @@ class ResidualNorm(nn.Module):
 
 class Int8Pointwise(nn.Module):
     """A 1x1 convolution or a linear layer in 8-bit integers, for inference (`functional.pointwise_int8`): weights as integers
-    with a scale for each output channel, every token of the input quantised by its largest channel."""
+    with a scale for each output channel, every token of the input quantised by its largest channel.  `layer` is on a CUDA
+    device; later changes of its weights do not reach the module."""
 
     def __init__(self, layer):
         super().__init__()
