@@ -255,6 +255,7 @@ static int clip_launch(const cvb_span* spans, int from, int to, bool scale, cons
   static thread_local ClipParams<N> P;
   P.partial = base.partial; P.norm = base.norm; P.max_norm = base.max_norm; P.partials = base.partials; P.kind = base.kind;
   P.writes_norm = base.writes_norm;
+  unsigned long long all = 0;
   unsigned chunks = 0;
   int count = 0;
   for (int i = from; i < to; ++i) {
@@ -267,7 +268,9 @@ static int clip_launch(const cvb_span* spans, int from, int to, bool scale, cons
     t.n_low = (unsigned)s.n; t.n_high = (unsigned short)(s.n >> 32);
     const bool vectors = (((size_t)s.in - t.ahead * in_size) & 15) == 0 && (((size_t)s.out - t.ahead * out_size) & 15) == 0;
     t.types = (unsigned short)((s.in_type == CVB_BF16) | (s.out_type == CVB_BF16) << 1 | vectors << 2);
-    chunks += (unsigned)((s.n + t.ahead + kChunk - 1) / kChunk);
+    all += (unsigned long long)(s.n + t.ahead + kChunk - 1) / kChunk;
+    if (all > 0x7fffffffull) return CVB_ERR_TOO_LARGE;
+    chunks = (unsigned)all;
   }
   P.count = count;
   P.chunks = chunks;

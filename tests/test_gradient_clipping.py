@@ -234,6 +234,7 @@ def test_c_abi_refusals():
     assert call(Span(16, 17, 4, 0, 1)) == -1
     assert call(Span(16, 16, 4, 0, 1)) == -1               # in place needs one type
     assert call(Span(16, 16, -1, 0, 0)) == -1
+    assert call(Span(16, 16, 1 << 45, 0, 0)) == -7
     assert call(Span(16, 16, 4, 3, 0)) == -1
     assert call(kind=3) == call(count=-1) == call(norm=None) == call(max_norm=-1.0) == call(max_norm=float("nan")) == -1
     assert call(work=None) == call(size=ws - 1) == -4

@@ -350,6 +350,39 @@ def test_streams_graphs_and_saved_tensors():
 
 
 @pytest.mark.gpu
+def test_a_captured_step():
+    """Forward and gradients captured into a graph and replayed on other inputs."""
+    t = _case("first", 64, 2, 30, 31, torch.float32, "layer", True, "image", True)
+    names = [n for n in NAMES if n in t]
+    static = {n: v.clone() for n, v in t.items()}
+    for n in names:
+        static[n].requires_grad_(True)
+
+    def step():
+        y, z = _call(static, "first", "layer", True)
+        return (y, z) + torch.autograd.grad((y, z), [static[n] for n in names], (static["dy"], static["dz"]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    other = _case("first", 64, 2, 30, 31, torch.float32, "layer", True, "image", True, seed=9)
+    with torch.no_grad():
+        for n, v in other.items():
+            static[n].copy_(v)
+    graph.replay()
+    torch.cuda.synchronize()
+    captured = [c.detach().clone() for c in captured]
+    for a, b in zip(captured, step()):
+        assert torch.equal(a, b.detach())
+
+
+@pytest.mark.gpu
 def test_saved_tensor_hooks_checkpointing_and_threads():
     """What the backward reads passes through saved-tensor hooks; a checkpoint runs the forward again; calls from several threads on
     streams of their own."""
