@@ -68,16 +68,17 @@ struct Seam {
     A.gate_kind = CVB_GATE_IMAGE;
     if (c.last && !empty) A.B = x0.size(0), A.HW = x0.numel() / C / A.B;
   }
+  // (no gradients are recorded here: the caller has none to record, or autograd's own function has switched them off)
   void lay_out() {
-    x = t[kX].detach().contiguous();
-    branch = t[kBranch].detach().contiguous();
+    x = t[kX].contiguous();
+    branch = t[kBranch].contiguous();
     A.x = x.data_ptr(); A.branch = branch.data_ptr();
     for (int i = kScale; i < kSeamTensors; ++i)
-      if (t[i].defined() && i != kGate) vec[i] = f32(t[i].detach());
+      if (t[i].defined() && i != kGate) vec[i] = f32(t[i]);
     A.scale = data<const float>(vec[kScale]); A.post_w = data<const float>(vec[kPostW]); A.post_b = data<const float>(vec[kPostB]);
     A.pre_w = data<const float>(vec[kPreW]); A.pre_b = data<const float>(vec[kPreB]);
-    if (A.gate_kind == CVB_GATE_FULL) gate = t[kGate].detach().contiguous();
-    if (A.gate_kind == CVB_GATE_IMAGE) gate = f32(t[kGate].detach());
+    if (A.gate_kind == CVB_GATE_FULL) gate = t[kGate].contiguous();
+    if (A.gate_kind == CVB_GATE_IMAGE) gate = f32(t[kGate]);
     A.gate = data<void>(gate);
     A.stream = stream(x);
   }
@@ -115,7 +116,7 @@ std::array<at::Tensor, kSeamTensors> seam_backward(Seam& s, const at::Tensor& st
     zero(0);
   } else {
     for (at::Tensor* t : {&dy, &dz}) {
-      if (t->defined()) *t = t->detach().to(s.x.scalar_type()).contiguous();
+      if (t->defined()) *t = t->to(s.x.scalar_type()).contiguous();
       if (t->defined() && t->sizes() != s.x.sizes()) throw Failed("a gradient must have the shape of its output");
     }
     auto& A = s.A;
@@ -406,9 +407,9 @@ struct Int8Weight {
     same_device(bias, x, "bias");
   }
   void lay_out() {
-    w = int8_rows(w.detach(), ld);
-    scale = f32(scale.detach());
-    if (bias.defined()) bias = f32(bias.detach());
+    w = int8_rows(w, ld);
+    scale = f32(scale);
+    if (bias.defined()) bias = f32(bias);
   }
 };
 
@@ -423,7 +424,7 @@ PyObject* py_quantize_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
     at::Tensor q, scale;
     {
       const Unlocked unlocked;
-      const at::Tensor x = x0.detach().contiguous();
+      const at::Tensor x = x0.contiguous();
       const int64_t padded = (t.K + 15) / 16 * 16;
       std::vector<int64_t> sizes = t.lead;
       scale = at::empty(sizes, x.options().dtype(at::kFloat).requires_grad(false));
@@ -461,7 +462,7 @@ PyObject* py_int8_product(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (out.numel()) {
         w.lay_out();
         long long ld;
-        const at::Tensor q = int8_rows(q0.detach().reshape({-1, t.K}), ld), scale = f32(s0.detach());
+        const at::Tensor q = int8_rows(q0.reshape({-1, t.K}), ld), scale = f32(s0);
         check(api.int8_product((const signed char*)q.data_ptr(), ld, (const float*)scale.data_ptr(), (const signed char*)w.w.data_ptr(),
                                w.ld, (const float*)w.scale.data_ptr(), data<const float>(w.bias), out.data_ptr(), t.B, t.HW, t.K, w.N,
                                last, bf16 ? CVB_BF16 : CVB_F32, stream(q0)),
@@ -487,7 +488,7 @@ PyObject* py_pointwise_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
       out = at::empty(t.result(w.N), x0.options().requires_grad(false));
       if (out.numel()) {
         w.lay_out();
-        const at::Tensor x = x0.detach().contiguous();
+        const at::Tensor x = x0.contiguous();
         const size_t ws = api.pointwise_int8_workspace(t.B, t.HW, t.K, w.N, t.last, io);
         at::Tensor work;
         if (ws) work = bytes_like(x, ws);
