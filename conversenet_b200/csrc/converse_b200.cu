@@ -795,6 +795,8 @@ static int check_int8(long long B, long long HW, int K, int io_dtype) {
   if (B < 1 || HW < 1 || K < 1 || (io_dtype != CVB_F32 && io_dtype != CVB_BF16)) return CVB_ERR_BAD_ARGUMENT;
   return K > 131072 || HW > 0x7fffff00ll / B ? CVB_ERR_TOO_LARGE : CVB_OK;
 }
+// one pixel an image: the layouts are the same, and tokens side by side fill a tile
+static bool int8_last(int channels_last, long long HW) { return channels_last != 0 || HW == 1; }
 static bool int8_rows(const void* p, long long ld, int K) { return p && (size_t)p % 16 == 0 && ld % 16 == 0 && ld >= K; }
 
 int cvb_quantize_tokens(const void* x, signed char* q, float* scale, long long B, long long HW, int K, long long ldq,
@@ -802,7 +804,7 @@ int cvb_quantize_tokens(const void* x, signed char* q, float* scale, long long B
   const int rc = check_int8(B, HW, K, io_dtype);
   if (rc != CVB_OK) return rc;
   if (!x || !scale || !int8_rows(q, ldq, K)) return CVB_ERR_BAD_ARGUMENT;
-  return i8::run_quantize(x, q, scale, B, HW, K, ldq, channels_last != 0, io_dtype, (cudaStream_t)stream);
+  return i8::run_quantize(x, q, scale, B, HW, K, ldq, int8_last(channels_last, HW), io_dtype, (cudaStream_t)stream);
 }
 
 int cvb_int8_product(const signed char* q, long long ldq, const float* scale, const signed char* w, long long ldw,
@@ -811,13 +813,13 @@ int cvb_int8_product(const signed char* q, long long ldq, const float* scale, co
   const int rc = check_int8(B, HW, K, io_dtype);
   if (rc != CVB_OK) return rc;
   if (!int8_rows(q, ldq, K) || !int8_rows(w, ldw, K) || !scale || !w_scale || !out || N < 1) return CVB_ERR_BAD_ARGUMENT;
-  return i8::run_product(q, ldq, scale, w, ldw, w_scale, bias, out, B, HW, K, N, channels_last != 0, io_dtype, sm_count(),
+  return i8::run_product(q, ldq, scale, w, ldw, w_scale, bias, out, B, HW, K, N, int8_last(channels_last, HW), io_dtype, sm_count(),
                          status_ptr(), (cudaStream_t)stream);
 }
 
 size_t cvb_pointwise_int8_workspace_bytes(long long B, long long HW, int K, int N, int channels_last, int io_dtype) {
   if (check_int8(B, HW, K, io_dtype) != CVB_OK || N < 1) return 0;
-  return i8::workspace(B, HW, K, N, channels_last != 0, io_dtype, sm_count());
+  return i8::workspace(B, HW, K, N, int8_last(channels_last, HW), io_dtype, sm_count());
 }
 
 int cvb_pointwise_int8(const void* x, const signed char* w, long long ldw, const float* w_scale, const float* bias, void* out,
@@ -826,9 +828,9 @@ int cvb_pointwise_int8(const void* x, const signed char* w, long long ldw, const
   const int rc = check_int8(B, HW, K, io_dtype);
   if (rc != CVB_OK) return rc;
   if (!x || !int8_rows(w, ldw, K) || !w_scale || !out || N < 1) return CVB_ERR_BAD_ARGUMENT;
-  const size_t need = i8::workspace(B, HW, K, N, channels_last != 0, io_dtype, sm_count());
+  const size_t need = i8::workspace(B, HW, K, N, int8_last(channels_last, HW), io_dtype, sm_count());
   if (need && (!workspace || (size_t)workspace % 16 || workspace_bytes < need)) return CVB_ERR_WORKSPACE;
-  return i8::run_pointwise(x, w, ldw, w_scale, bias, out, B, HW, K, N, channels_last != 0, io_dtype, workspace, sm_count(),
+  return i8::run_pointwise(x, w, ldw, w_scale, bias, out, B, HW, K, N, int8_last(channels_last, HW), io_dtype, workspace, sm_count(),
                            status_ptr(), (cudaStream_t)stream);
 }
 

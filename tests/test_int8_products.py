@@ -191,6 +191,23 @@ def test_extremes():
 
 
 @pytest.mark.gpu
+def test_many_small_images_and_other_ranks():
+    """Images of one pixel, which are tokens side by side, and of a few; tokens with more dimensions."""
+    wq, ws = CF.quantize_weight(torch.randn(40, 64, device="cuda"))
+    x = _features((30000, 64, 1, 1), True, torch.float32, 2)
+    y = CF.pointwise_int8(x, wq, ws)
+    assert torch.equal(y.flatten(1), CF.pointwise_int8(x.flatten(1), wq, ws, data_format="channels_last"))
+    q, s = CF.quantize_tokens(x)
+    assert q.shape == (30000, 1, 1, 64) and torch.equal(CF.int8_product(q, s, wq, ws, data_format="channels_first"), y)
+    x = _features((3000, 64, 1, 2), True, torch.bfloat16, 3)
+    q, scale = _integers(_rows(x, True))
+    _check_product(CF.pointwise_int8(x, wq, ws), q, scale, wq, ws, None, True)
+    x = _features((2, 3, 5, 7, 64), False, torch.float32, 4)
+    y = CF.pointwise_int8(x, wq, ws, data_format="channels_last")
+    assert y.shape == (2, 3, 5, 7, 40) and torch.equal(y.view(-1, 40), CF.pointwise_int8(x.view(-1, 64), wq, ws, data_format="channels_last"))
+
+
+@pytest.mark.gpu
 def test_module_streams_and_graphs():
     torch.manual_seed(0)
     conv = torch.nn.Conv2d(70, 33, 1).cuda()

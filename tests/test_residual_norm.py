@@ -350,6 +350,39 @@ def test_streams_graphs_and_saved_tensors():
 
 
 @pytest.mark.gpu
+def test_many_images_the_widest_and_other_ranks():
+    t = _case("first", 8, 70000, 2, 1, torch.float32, "layer", True, "image", True)          # more images than a grid's second axis
+    names = [n for n in NAMES if n in t]
+    for n in names:
+        t[n].requires_grad_(True)
+    y, z = _call(t, "first", "layer", True)
+    d = {n: v.detach().double().requires_grad_(n in names) for n, v in t.items()}
+    y64, z64 = _formula(d, "first", "layer", True)
+    _close(y, y64, 1, "y")
+    _close(z, z64, 1, "z")
+    got = torch.autograd.grad((y, z), [t["gate"], t["scale"], t["pre_weight"]], (t["dy"], t["dz"]))
+    ref = torch.autograd.grad((y64, z64), [d["gate"], d["scale"], d["pre_weight"]], (d["dy"], d["dz"]))
+    for a, b in zip(got, ref):
+        assert float((a.double() - b).norm() / b.norm()) <= 1e-5
+    t = _case("first", 16384, 1, 3, 5, torch.bfloat16, "rms", True, "full", True)
+    y, z = _call(t, "first", "rms", True)
+    y64, z64 = _formula({n: v.double() for n, v in t.items()}, "first", "rms", True)
+    _close(y, y64, 1, "y")
+    _close(z, z64, 1, "z")
+    # (T,C), and tokens of three dimensions with a gate for each image
+    t = _case("last", 48, 3, 4, 6, torch.float32, "layer", True, "image", True)
+    y, z = _call(t, "last", "layer", True)
+    u = dict(t, x=t["x"].view(3, 4, 6, 48), branch=t["branch"].view(3, 4, 6, 48), gate=t["gate"].view(3, 1, 1, 48))
+    for a, b in zip(_call(u, "last", "layer", True), (y, z)):
+        assert torch.equal(a.view_as(b), b)
+    flat = {n: v for n, v in t.items() if n != "gate"}
+    y, z = _call(flat, "last", "layer", False)
+    u = dict(flat, x=t["x"].reshape(-1, 48), branch=t["branch"].reshape(-1, 48))
+    for a, b in zip(_call(u, "last", "layer", False), (y, z)):
+        assert torch.equal(a.view_as(b), b)
+
+
+@pytest.mark.gpu
 def test_a_captured_step():
     """Forward and gradients captured into a graph and replayed on other inputs."""
     t = _case("first", 64, 2, 30, 31, torch.float32, "layer", True, "image", True)
