@@ -468,6 +468,7 @@ static int quantize_last(QuantParams& P, cudaStream_t st) {
                 : launch_chained(quant_last_kernel<IO, NV, false>, grid, 256, 0, st, P);
   };
   return each == 1   ? go(std::integral_constant<int, 1>())
+         : each == 2 ? go(std::integral_constant<int, 2>())
          : each <= 4 ? go(std::integral_constant<int, 4>())
                      : go(std::integral_constant<int, 16>());
 }

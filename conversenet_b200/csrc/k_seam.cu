@@ -1268,6 +1268,9 @@ static int cf_fwd_any(Params& P, int sms, cudaStream_t st) {
   if (P.C <= 64 && several) return along4 ? cf_fwd<IO, 8, 4, true, 256, 2>(P, st) : cf_fwd<IO, 8, 4, false, 256, 2>(P, st);
   if (P.C <= 96 && several) return along2 ? cf_fwd<IO, 8, 2, true, 384, 2>(P, st) : cf_fwd<IO, 8, 2, false, 384, 2>(P, st);
   if (P.C <= 128 && several) return along4 ? cf_fwd<IO, 8, 4, true, 512, 1>(P, st) : cf_fwd<IO, 8, 2, false, 512, 2>(P, st);
+  // Up to 256 sixteen channels a thread: two pixels as vectors (4 x 256 x 16384 fp32 66 us; one pixel in two blocks of 512 threads 78;
+  // eight channels in one block of 1024 99), or one where rows allow none (5 x 184 x 18221 bf16 97 us, two pixels 118, eight channels 130)
+  if (P.C <= 256 && several) return along2 ? cf_fwd<IO, 16, 2, true, 512, 1>(P, st) : cf_fwd<IO, 16, 1, true, 512, 2>(P, st);
   if (P.C <= 256) return cf_fwd<IO, 8, 1, true, 1024, 1>(P, st);
   if (P.C <= 1024) return cf_fwd<IO, 32, 1, true, 1024, 1>(P, st);
   P.tiles = ceil_div(P.HW, 32);

@@ -112,6 +112,10 @@ CASES = [
     ("first", 96, 2, 75, 87, "bf16", "layer", True, "image", True),
     ("first", 96, 1, 128, 128, "bf16", "layer", False, "full", True),
     ("first", 200, 2, 13, 17, "fp32", "rms", True, "image", False),
+    ("first", 128, 1, 111, 97, "bf16", "layer", True, "none", True),
+    ("first", 120, 1, 100, 100, "fp32", "layer", True, "full", True),
+    ("first", 200, 1, 111, 97, "bf16", "layer", True, "image", True),       # sixteen channels a thread
+    ("first", 256, 1, 100, 98, "fp32", "rms", True, "full", True),
     ("first", 300, 2, 9, 11, "bf16", "layer", True, "full", True),          # wide: values are read again
     ("first", 1030, 1, 5, 7, "fp32", "layer", True, "image", True),
     ("first", 1, 2, 5, 7, "fp32", "rms", True, "none", True),
