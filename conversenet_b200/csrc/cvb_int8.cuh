@@ -5,7 +5,8 @@
 // exact product x r to an integer, to an even one from a half, and its bits end in it.
 //
 // fp32: r is 127 / a rounded to nearest, and x r off by less than 127 . 2^-24 = 7.6e-6.  Where it lies nearer than 2e-5 to a half,
-// m + 1/2 (4 values in 100000), the sign of 254 |x| - (2 m + 1) a decides, each product as a sum of two fp32 numbers.
+// m + 1/2 (4 values in 100000), the sign of 254 |x| - (2 m + 1) a decides, each product as a sum of two fp32 numbers.  So that 254 a is
+// an fp32 number and no product loses digits, x and a are multiplied by a power of two first where a lies outside [2^-100, 2^100].
 //
 // bf16: r is rounded up, and that is enough.  With x = X 2^p, a = A 2^q, X, A integers up to 255, e = p - q <= 0: unless t is a half
 // it is at least 2^e / (2 A) >= 2^e / 510 away from one, while x r exceeds t by less than t 2^-23 <= 255 . 2^e . 2^-23.  If t is
@@ -79,32 +80,33 @@ __device__ __forceinline__ uint32_t nearest_bytes(float x0, float x1, float x2, 
   }
   return low_bytes(u, v);
 }
-// tokens whose 127 / a is no fp32 number, scaled; 0 where an infinity or a NaN is among the values
-static __device__ __noinline__ uint32_t nearest_bytes_of_tiny(float x0, float x1, float x2, float x3, float a) {
+// Tokens of very small or very large values, scaled by 2^100 or 2^-100, which leaves every integer as it is: exact, but for values of
+// a large token that leave fp32's range below, which are 0.  0 where an infinity or a NaN is among the values.
+static __device__ __noinline__ uint32_t nearest_bytes_scaled(float x0, float x1, float x2, float x3, float a) {
   if (!(a < INFINITY)) return 0;
-  const float up = 0x1p100f, top = a * up;
+  const float by = a < 1.f ? 0x1p100f : 0x1p-100f, top = a * by;
   bool left;
-  return nearest_bytes(x0 * up, x1 * up, x2 * up, x3 * up, top, __fdiv_rn(127.f, top), false, left);
+  return nearest_bytes(x0 * by, x1 * by, x2 * by, x3 * by, top, __fdiv_rn(127.f, top), false, left);
 }
 
 template <bool BF16>
 struct Quantiser {
   float a, r;
-  bool hard;          // 127 / a is no fp32 number; or an infinity or a NaN among the values (0, the scale says so)
+  bool hard;          // 127 / a or 254 a may be no fp32 number; or an infinity or a NaN among the values (0, the scale says so)
   __device__ __forceinline__ explicit Quantiser(float largest_magnitude) : a(largest_magnitude) {
-    hard = !(a < INFINITY) || (a < 0x1p-100f && a != 0.f);
+    hard = !(a <= (BF16 ? 0x1.fffffep127f : 0x1p100f)) || (a < 0x1p-100f && a != 0.f);          // (bf16 forms no 254 a)
     r = hard || a == 0.f ? 0.f : BF16 ? __fdiv_ru(127.f, a) : __fdiv_rn(127.f, a);
   }
   __device__ __forceinline__ float scale() const { return a < INFINITY ? __fdiv_rn(a, 127.f) : __uint_as_float(0x7fffffffu); }
   __device__ __forceinline__ uint32_t four(float x0, float x1, float x2, float x3) const {
     if (BF16) {
-      if (hard) return nearest_bytes_of_tiny(x0, x1, x2, x3, a);
+      if (hard) return nearest_bytes_scaled(x0, x1, x2, x3, a);
       const float2 rr = make_float2(r, r), mm = make_float2(kRounder, kRounder);
       return low_bytes(fma2(make_float2(x0, x1), rr, mm), fma2(make_float2(x2, x3), rr, mm));
     }
     bool left;
     const uint32_t w = nearest_bytes(x0, x1, x2, x3, a, r, hard, left);
-    return left ? nearest_bytes_of_tiny(x0, x1, x2, x3, a) : w;
+    return left ? nearest_bytes_scaled(x0, x1, x2, x3, a) : w;
   }
 };
 

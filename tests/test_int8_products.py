@@ -342,3 +342,42 @@ def test_c_abi_refusals():
     assert lib.cvb_pointwise_int8_workspace_bytes(1, 100, 64, 8, 0, 0) == 0          # quantised on the way
     assert lib.cvb_pointwise_int8(p, p, 304, p, None, p, 1, 100, 300, 8, 1, 0, None, 0, None) == -4
     assert lib.cvb_pointwise_int8(p, p, 304, p, None, p, 1, 100, 300, 8, 1, 0, p, need - 1, None) == -4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("K", [3, 64, 128, 250, 600, 5000])
+@pytest.mark.parametrize("power", [95, 96, 97, 103, 104])
+def test_integers_of_large_tokens_are_the_nearest(K, dtype, power):
+    """Borders between two integers in tokens up to the largest finite number: the constructions of the test above times a power of
+    two, which is exact (the largest magnitudes are 2^23 to 2^24 times it)."""
+    dtype = DTYPES[dtype]
+    g = torch.Generator(device="cuda").manual_seed(K + power)
+    T = 2000 if K <= 600 else 240
+    up = 2.0 ** power
+    top = torch.randint(1 << 23, 1 << 24, (T, 1), device="cuda", generator=g).float()
+    top[0] = (1 << 24) - 1
+    odd = 2 * torch.randint(-127, 127, (T, K), device="cuda", generator=g).double() + 1
+    near = (odd * top.double() / 254).float()
+    beside = torch.nextafter(near, torch.randn(T, K, device="cuda", generator=g) * 1e9)
+    halves = 131072.0 * (torch.randint(-126, 126, (T, K), device="cuda", generator=g) + 0.5)
+    half = torch.where(torch.rand(T, K, device="cuda", generator=g) < 0.5, 0.5 * top, -0.5 * top)
+    near[:, 0] = beside[:, 0] = half[:, 0] = top[:, 0]
+    halves[:, 0] = 127 * 131072.0
+    for name, x in (("near", near), ("beside", beside), ("halves", halves), ("half of the largest", half)):
+        if dtype == torch.bfloat16:          # (rounded first: the largest would become an infinity)
+            x = x.clamp(-16711680.0, 16711680.0).to(dtype).float()
+        x = (x * up).to(dtype)
+        assert bool(torch.isfinite(x).all())
+        ref, scale = _integers(x)
+        q, s = CF.quantize_tokens(x, "channels_last")
+        assert torch.equal(q.double(), ref), name
+        assert bool(((s.double() - scale[:, 0]).abs() <= 2.0 ** -24 * scale[:, 0]).all()), name
+        planes = x.t().reshape(1, K, T // 40, 40).contiguous()
+        q2, s2 = CF.quantize_tokens(planes)
+        assert torch.equal(q2.reshape(T, K), q) and torch.equal(s2.reshape(T), s), name
+        if K <= 128:
+            # on the way to a product: unit weights of 2^-8, so that no result is beyond fp32
+            out = CF.pointwise_int8(planes, torch.eye(K, dtype=torch.int8, device="cuda"), torch.full((K,), 2.0 ** -8, device="cuda"))
+            want = ((q.float() * 2.0 ** -8) * s[:, None]).to(dtype)
+            assert torch.equal(out.reshape(K, T).t(), want), name
