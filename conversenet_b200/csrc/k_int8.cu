@@ -14,6 +14,7 @@
 #include <cuda.h>
 
 #include <atomic>
+#include <climits>
 #include <type_traits>
 
 #include "../../include/converse_b200.h"
@@ -190,6 +191,7 @@ __global__ void __launch_bounds__(256, NV == 16 ? 2 : 3) quant_last_kernel(const
 
 // ------------------------------------------------------------------ product
 constexpr int kM = 128, kBK = 128;                     // rows of L in a tile; bytes of K in a stage
+constexpr int kMostK = 131072;                         // sums from -127 . 128 . 2^17 to 2^31
 constexpr int kEpilogueWarps = 8, kThreads = 32 * (4 + kEpilogueWarps);
 constexpr int kPolls = 1 << 20;
 
@@ -388,6 +390,10 @@ product_kernel(const __grid_constant__ CUtensorMap mapL, const __grid_constant__
         for (int c = 0; c < left; c += 32) {
           int v[32];
           tmem_ld32i(tmem + acc * NT + half * (NT / 2) + c + ((uint32_t)(quadrant * 32) << 16), v);
+          if (P.K == kMostK) {          // 2^31 = 131072 . 128 . 128 came out as -2^31, which no other sum is: 2^31 - 1 is 2^31 in fp32
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = v[j] == INT_MIN ? INT_MAX : v[j];
+          }
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             const float4 s4 = *(const float4*)(rs + c + j);

@@ -381,3 +381,22 @@ def test_integers_of_large_tokens_are_the_nearest(K, dtype, power):
             out = CF.pointwise_int8(planes, torch.eye(K, dtype=torch.int8, device="cuda"), torch.full((K,), 2.0 ** -8, device="cuda"))
             want = ((q.float() * 2.0 ** -8) * s[:, None]).to(dtype)
             assert torch.equal(out.reshape(K, T).t(), want), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["first", "last"])
+def test_the_largest_sum_of_all(layout):
+    """131072 products of -128 and -128 are 2^31, one more than a signed 32-bit integer holds; every one of these sums is an fp32
+    number."""
+    K = 131072
+    q = torch.full((1, 1, 3, K), -128, dtype=torch.int8, device="cuda")
+    q[0, 0, 1] = 127
+    q[0, 0, 2, K // 2:] = 0
+    w = torch.full((300, K), -128, dtype=torch.int8, device="cuda")
+    w[1::3] = 127
+    w[2::3, :] = 0
+    out = CF.int8_product(q, torch.ones(1, 1, 3, device="cuda"), w, torch.ones(300, device="cuda"), data_format="channels_" + layout)
+    want = torch.tensor([[-128.0 * -128, -128 * 127, 0], [127 * -128, 127 * 127, 0], [-64 * -128, -64 * 127, 0]],
+                        dtype=torch.float64, device="cuda").repeat(1, 100) * K
+    assert float(want.max()) == 2.0 ** 31 and torch.equal(want.float().double(), want)
+    assert torch.equal(out.permute(0, 2, 3, 1).reshape(3, 300).double() if layout == "first" else out.reshape(3, 300).double(), want)
