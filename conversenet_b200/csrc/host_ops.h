@@ -57,13 +57,14 @@ struct Seam {
     if (!c.last) A.B = x0.size(0), A.HW = x0.size(2) * x0.size(3);
     const at::Tensor& g = t[kGate];
     if (!g.defined()) return;
-    if (g.sizes() == x0.sizes()) {
+    bool image = g.dim() == x0.dim() && g.size(0) == x0.size(0);
+    for (int64_t d = 1; image && d < x0.dim(); ++d) image = g.size(d) == (d == (c.last ? x0.dim() - 1 : 1) ? C : 1);
+    // (images of one pixel: both, and of any type as an image's gate)
+    if (g.sizes() == x0.sizes() && (!image || g.scalar_type() == x0.scalar_type())) {
       if (g.scalar_type() != x0.scalar_type()) throw Failed("a gate for each element must have the type of x");
       A.gate_kind = CVB_GATE_FULL;
       return;
     }
-    bool image = g.dim() == x0.dim() && g.size(0) == x0.size(0);
-    for (int64_t d = 1; image && d < x0.dim(); ++d) image = g.size(d) == (d == (c.last ? x0.dim() - 1 : 1) ? C : 1);
     if (!image) throw Failed("gate must have the shape of x, or hold a value for each image and channel");
     A.gate_kind = CVB_GATE_IMAGE;
     if (c.last && !empty) A.B = x0.size(0), A.HW = x0.numel() / C / A.B;

@@ -564,3 +564,45 @@ def test_c_abi_refusals():
     assert bwd(C=5000) == -7
     assert lib.cvb_residual_norm_workspace_bytes(64, 8, 0) >= 16 * 64
     assert lib.cvb_residual_norm_workspace_bytes(0, 8, 0) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gate_dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(3, 40, 1, 1), (3, 1, 40), (5, 40), (2, 1, 1, 40)], ids=str)
+def test_a_gate_for_each_image_of_one_pixel(shape, dtype, gate_dtype):
+    """Its shape is that of x; its type is its own, as at every other size."""
+    first = shape[1] == 40 and len(shape) == 4
+    layout, C = "first" if first else "last", 40
+    g = torch.Generator(device="cuda").manual_seed(2)
+    t = {n: torch.randn(shape, device="cuda", generator=g).to(dtype) for n in ("x", "branch", "dy", "dz")}
+    t["gate"] = torch.randn(shape, device="cuda", generator=g).to(gate_dtype)
+    for n in ("scale", "post_weight", "post_bias", "pre_weight", "pre_bias"):
+        t[n] = 0.5 + torch.rand(C, device="cuda", generator=g)
+    d = {n: v.double() for n, v in t.items()}
+    for n in NAMES:
+        t[n].requires_grad_(True)
+        d[n].requires_grad_(True)
+    out = _call(t, layout, "layer", True)
+    ref = _formula(d, layout, "layer", True)
+    dim = 1 if first else -1
+    for a, b in zip(out, ref):
+        _close(a, b, dim, "outputs")
+    got = torch.autograd.grad(out, [t[n] for n in NAMES], (t["dy"], t["dz"]))
+    want = torch.autograd.grad(ref, [d[n] for n in NAMES], (d["dy"], d["dz"]))
+    tops = _before_cancelling(d, layout, "layer", True)
+    with torch.no_grad():
+        # A vector's gradient is a sum of at most five terms, each off by 96 . 2^-24 of the largest value it is formed from (dz; or the
+        # gradient of y, at most the branch's scale and gate times the token's top) times what is normalised (|h| <= sqrt(C)) or p.
+        top = tops["x"].max() * (d["scale"].max() * 1.0)
+        p = ((d["post_weight"].max() * C ** 0.5) + d["post_bias"].max())
+        sizes = {"pre_bias": d["dz"].abs().max(), "pre_weight": d["dz"].abs().max() * C ** 0.5, "post_bias": top,
+                 "post_weight": top * C ** 0.5, "scale": tops["x"].max() * p}
+    for n, a, b in zip(NAMES, got, want):
+        assert a.dtype == t[n].dtype and a.shape == t[n].shape
+        if n in tops:
+            over = (a.double() - b).abs() - 96 * 2.0 ** -24 * tops[n] - (torch.finfo(a.dtype).eps / 2 + 2.0 ** -24) * b.abs() - \
+                (2.0 ** -25 if a.dtype == torch.float16 else 0)                # (half of fp16's smallest number)
+        else:
+            over = (a.double() - b).abs() - 160 * 2.0 ** -24 * 5 * sizes[n]
+        assert float(over.max()) <= 0, (n, float(over.max()))
