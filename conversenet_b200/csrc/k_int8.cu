@@ -389,6 +389,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapL, const __grid_constant__
         IO* out = (IO*)P.out + tile.image * P.image_stride + (long long)c0 * P.ldc + r;
         for (int c = 0; c < left; c += 32) {
           int v[32];
+          __syncwarp();          // (not every lane has stored what is before)
           tmem_ld32i(tmem + acc * NT + half * (NT / 2) + c + ((uint32_t)(quadrant * 32) << 16), v);
           if (P.K == kMostK) {          // 2^31 = 131072 . 128 . 128 came out as -2^31, which no other sum is: 2^31 - 1 is 2^31 in fp32
 #pragma unroll
@@ -412,6 +413,7 @@ product_kernel(const __grid_constant__ CUtensorMap mapL, const __grid_constant__
           }
         }
       }
+      __syncwarp();
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&free_[acc]);

@@ -123,6 +123,7 @@ __global__ void __launch_bounds__(kPlaneThreads* kPlaneGroups, 1) planes_kernel(
     for (int i = 0; i < groups; ++i) mbar_init(&bars[i], 1);
     mbar_fence_init();
   }
+  __syncwarp();
   if (threadIdx.x < 32) tc::tmem_alloc(&tmem_base, groups == 1 ? 256 : 512);
   tc::fence_proxy_async();
   tc::fence_before_sync();
@@ -164,6 +165,7 @@ __global__ void __launch_bounds__(kPlaneThreads* kPlaneGroups, 1) planes_kernel(
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) w[j] = q.four(v[16 * i + 4 * j], v[16 * i + 4 * j + 1], v[16 * i + 4 * j + 2], v[16 * i + 4 * j + 3]);
+      __syncwarp();          // (a value next to a border took some lanes another way; the store is one of the whole warp)
       plane_st4(lanes + 128 + half * (CH / 4) + 4 * i, w[0], w[1], w[2], w[3]);
     }
     tc::tmem_wait_st();
@@ -186,6 +188,7 @@ __global__ void __launch_bounds__(kPlaneThreads* kPlaneGroups, 1) planes_kernel(
       IO* out = (IO*)P.out + (b * P.N + n0) * P.HW + px;
       for (int c = 16 * half; c < cols; c += 32) {
         int s[16];
+        __syncwarp();          // (lanes behind the last pixel store nothing, and the load is one of the whole warp)
         plane_ld16(lanes + c, s);
         tc::tmem_wait_ld();
         IO* to = out + c * P.HW;
@@ -206,6 +209,7 @@ __global__ void __launch_bounds__(kPlaneThreads* kPlaneGroups, 1) planes_kernel(
           }
         }
       }
+      __syncwarp();
     }
   }
   if (!alive && lane == 0 && P.status) *P.status = 1;

@@ -400,3 +400,19 @@ def test_the_largest_sum_of_all(layout):
                         dtype=torch.float64, device="cuda").repeat(1, 100) * K
     assert float(want.max()) == 2.0 ** 31 and torch.equal(want.float().double(), want)
     assert torch.equal(out.permute(0, 2, 3, 1).reshape(3, 300).double() if layout == "first" else out.reshape(3, 300).double(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [17, 128, 140])
+@pytest.mark.parametrize("HW", [2, 5, 31, 33, 95, 127, 129, 300])
+def test_planes_that_end_inside_a_warp(HW, K):
+    """The last pixels of each image leave some of a warp's lanes without one, in several groups of output channels."""
+    B, N = 3, 305
+    g = torch.Generator(device="cuda").manual_seed(HW + K)
+    x = torch.randn(B, K, 1, HW, device="cuda", generator=g)
+    wq, ws = CF.quantize_weight(torch.randn(N, K, device="cuda", generator=g))
+    q, scale = _integers(_rows(x, True))
+    _check_product(CF.pointwise_int8(x, wq, ws), q, scale, wq, ws, None, True)
+    qt, st = CF.quantize_tokens(x)
+    for fmt in ("channels_first", "channels_last"):
+        _check_product(CF.int8_product(qt, st, wq, ws, data_format=fmt), q, scale, wq, ws, None, fmt == "channels_first")
