@@ -1241,6 +1241,11 @@ static bool aligned(const Params& P, size_t to) {
     if ((size_t)p % to) return false;
   return true;
 }
+// pixels of a thread as vectors of each tensor, and of the means and spreads
+template <typename IO>
+static bool pixels_aligned(const Params& P, int pixels) {
+  return P.HW % pixels == 0 && aligned(P, pixels * sizeof(IO)) && (size_t)P.stats % (pixels * sizeof(float)) == 0;
+}
 static bool vectors_aligned(const Params& P) {
   const void* all[] = {P.scale, P.post_w, P.post_b, P.pre_w, P.pre_b, P.gate_kind == kGateImage ? P.gate : nullptr};
   for (const void* p : all)
@@ -1264,7 +1269,7 @@ static int cf_fwd_any(Params& P, int sms, cudaStream_t st) {
   // to 64 channels (two blocks an SM).  Up to 96 two, with two blocks of 384 threads (4 x 96 x 65536 fp32: 79 us, four pixels 92);
   // up to 128 four as vectors (118 us, two 114; bf16 102 and 107), two where they are 32 apart (bf16 120 us, four 161).
   const bool several = P.tokens >= (long long)64 * sms;
-  const bool along2 = P.HW % 2 == 0 && aligned(P, 2 * sizeof(IO)), along4 = P.HW % 4 == 0 && aligned(P, 4 * sizeof(IO));
+  const bool along2 = pixels_aligned<IO>(P, 2), along4 = pixels_aligned<IO>(P, 4);
   if (P.C <= 64 && several) return along4 ? cf_fwd<IO, 8, 4, true, 256, 2>(P, st) : cf_fwd<IO, 8, 4, false, 256, 2>(P, st);
   if (P.C <= 96 && several) return along2 ? cf_fwd<IO, 8, 2, true, 384, 2>(P, st) : cf_fwd<IO, 8, 2, false, 384, 2>(P, st);
   if (P.C <= 128 && several) return along4 ? cf_fwd<IO, 8, 4, true, 512, 1>(P, st) : cf_fwd<IO, 8, 2, false, 512, 2>(P, st);
@@ -1342,8 +1347,8 @@ static int cf_bwd(Params& P, int sms, cudaStream_t st) {
 template <typename IO, bool GATED>
 static int cf_bwd_any(Params& P, int sms, cudaStream_t st) {
   // as the forward: four pixels a thread (registers for 64 channels in a block of 256), or two
-  const bool four = P.tokens >= (long long)64 * sms, along4 = P.HW % 4 == 0 && aligned(P, 4 * sizeof(IO));
-  const bool along = P.HW % 2 == 0 && aligned(P, 2 * sizeof(IO));
+  const bool four = P.tokens >= (long long)64 * sms, along4 = pixels_aligned<IO>(P, 4);
+  const bool along = pixels_aligned<IO>(P, 2);
   if (P.C <= 64 && four) return along4 ? cf_bwd<IO, 4, true, GATED, 256, 1>(P, sms, st) : cf_bwd<IO, 4, false, GATED, 256, 1>(P, sms, st);
   if (P.C <= 128) return along ? cf_bwd<IO, 2, true, GATED, 512, 1>(P, sms, st) : cf_bwd<IO, 2, false, GATED, 512, 1>(P, sms, st);
   return cf_bwd<IO, 1, true, GATED, 1024, 1>(P, sms, st);

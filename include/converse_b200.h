@@ -346,6 +346,7 @@ int cvb_tap_gradient(const float* g_full, const float* r, float* out, int nseg, 
  *   tensors  : channels_last 0: (B,C,HW); 1: (B,HW,C); contiguous, io_dtype
  *   gate     : CVB_GATE_FULL like branch; CVB_GATE_IMAGE (B,C) fp32
  *   stats    : 4 B HW floats kept for the gradients, or NULL
+ * Every address at a boundary of its elements; tensors, vectors and stats at 16-byte boundaries move in wider pieces.
  * Backward, from dy = dL/dy and dz = dL/dz (either may be NULL), reading x (where dz is given), branch, gate and stats:
  * dx, dbranch, dgate (of the gate's layout and type) and the gradients of the vectors (each may be NULL).
  * C: up to 16384; backward in channels_first up to 4096 (CVB_ERR_TOO_LARGE).  The workspace is needed by the backward only.

@@ -606,3 +606,44 @@ def test_a_gate_for_each_image_of_one_pixel(shape, dtype, gate_dtype):
         else:
             over = (a.double() - b).abs() - 160 * 2.0 ** -24 * 5 * sizes[n]
         assert float(over.max()) <= 0, (n, float(over.max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("C,HW", [(24, 96), (24, 9600), (80, 9600), (120, 9600), (24, 9599)])
+def test_c_abi_stats_that_begin_anywhere(C, HW, dtype):
+    """Means and spreads kept at any float of a caller's buffer, read by the gradients there, and nothing written beside them."""
+    from conversenet_b200 import _cabi
+    lib = _cabi.load()
+    t = _case("first", C, 1, HW, 1, dtype, "layer", True, "none", True)
+    vec = dict(scale="scale", post_w="post_weight", post_b="post_bias", pre_w="pre_weight", pre_b="pre_bias")
+    got = []
+    for offset in (0, 1, 2, 3):
+        room = torch.full((4 * HW + 8,), 7.0, device="cuda")
+        o = {n: torch.empty_like(t["x"]) for n in ("y", "z", "dx", "dbranch")}
+        a = _arguments(x=t["x"], branch=t["branch"], dy=t["dy"], dz=t["dz"], **{k: t[n] for k, n in vec.items()}, **o)
+        a.B, a.HW, a.C, a.eps, a.io_dtype = 1, HW, C, EPS, int(dtype == torch.bfloat16)
+        a.stats, a.stream = room[4 + offset:].data_ptr(), torch.cuda.current_stream().cuda_stream
+        assert lib.cvb_residual_norm_fwd(ctypes.byref(a)) == 0
+        assert lib.cvb_residual_norm_bwd(ctypes.byref(a)) == 0
+        assert bool((room[:4 + offset] == 7).all()) and bool((room[4 + offset + 4 * HW:] == 7).all())
+        got.append([room[4 + offset:4 + offset + 4 * HW].clone(), *o.values()])
+    for other in got[1:]:
+        for a, b in zip(got[0], other):
+            # other pixels a thread, the same channels and order of sums: fp32 roundings at most, and a neighbour in the tensors' type
+            a, b = a.double(), b.double()
+            eps = torch.finfo(dtype).eps
+            assert bool(((a - b).abs() <= eps * a.abs() + 1e-5 * a.abs().max()).all())
+
+
+def _arguments(**tensors):
+    class Args(ctypes.Structure):
+        _fields_ = ([(n, ctypes.c_void_p) for n in ("x", "branch", "gate", "y", "z", "scale", "post_w", "post_b", "pre_w", "pre_b",
+                                                    "stats", "dy", "dz", "dx", "dbranch", "dgate", "dscale", "dpost_w", "dpost_b",
+                                                    "dpre_w", "dpre_b")] +
+                    [("B", ctypes.c_longlong), ("HW", ctypes.c_longlong)] +
+                    [(n, ctypes.c_int) for n in ("C", "channels_last", "rms", "gate_kind", "gate_act", "io_dtype")] +
+                    [("eps", ctypes.c_float), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+                     ("stream", ctypes.c_void_p)])
+
+    return Args(**{n: v.data_ptr() for n, v in tensors.items()})
