@@ -43,6 +43,10 @@ static const StaticEntry kStatic[] = {
 #undef CVB_STATIC
 };
 
+// every address at a boundary of `size` bytes
+template <class... T>
+bool at_elements(size_t size, const T*... p) { return (((size_t)p % size == 0) && ...); }
+
 // Device word set by a kernel whose bounded wait gave up (one per device).
 __device__ int g_device_status;
 int* status_ptr() {
@@ -722,6 +726,11 @@ static int seam_params(const cvb_residual_norm_args& A, bool backward, seam::Par
   if (A.gate_kind < CVB_GATE_NONE || A.gate_kind > CVB_GATE_IMAGE || (A.gate_kind != CVB_GATE_NONE) != (A.gate != nullptr))
     return CVB_ERR_BAD_ARGUMENT;
   if ((A.post_b && !A.post_w) || (A.pre_b && !A.pre_w) || !(A.eps >= 0.f)) return CVB_ERR_BAD_ARGUMENT;
+  const size_t e = A.io_dtype == CVB_BF16 ? 2 : 4;
+  if (!at_elements(e, A.x, A.branch, A.y, A.z, A.dy, A.dz, A.dx, A.dbranch) ||
+      !at_elements(A.gate_kind == CVB_GATE_FULL ? e : sizeof(float), A.gate, A.dgate) ||
+      !at_elements(sizeof(float), A.scale, A.post_w, A.post_b, A.pre_w, A.pre_b, A.stats, A.dscale, A.dpost_w, A.dpost_b, A.dpre_w, A.dpre_b))
+    return CVB_ERR_BAD_ARGUMENT;
   if (A.C > 16384) return CVB_ERR_TOO_LARGE;
   memset(&P, 0, sizeof(P));
   P.x = A.x; P.branch = A.branch; P.gate = A.gate; P.y = A.y; P.z = A.z;
@@ -764,7 +773,9 @@ int cvb_residual_norm_bwd(const cvb_residual_norm_args* args) {
   if (!P.branch && (P.dbranch || P.dgate || P.dscale || P.dpost_w || P.dpost_b)) return CVB_ERR_BAD_ARGUMENT;
   if (!P.dx && !P.dbranch && !P.dgate && !sums) return CVB_ERR_BAD_ARGUMENT;
   if (sums) {
-    if (!A.workspace || A.workspace_bytes < cvb_residual_norm_workspace_bytes(A.C, A.B, A.gate_kind)) return CVB_ERR_WORKSPACE;
+    if (!A.workspace || !at_elements(sizeof(float), A.workspace) ||
+        A.workspace_bytes < cvb_residual_norm_workspace_bytes(A.C, A.B, A.gate_kind))
+      return CVB_ERR_WORKSPACE;
     P.partial = (float*)A.workspace;
   }
   P.max_parts = seam::most_parts(A.C, A.B, A.gate_kind, sm_count());

@@ -647,3 +647,35 @@ def _arguments(**tensors):
                      ("stream", ctypes.c_void_p)])
 
     return Args(**{n: v.data_ptr() for n, v in tensors.items()})
+
+
+def test_c_abi_addresses():
+    from conversenet_b200 import _cabi
+
+    lib = _cabi.load()
+    one = 16                                   # never dereferenced: validation fails first
+
+    def fwd(**change):
+        a = _arguments()
+        for k, v in dict(dict(x=one, branch=one, y=one, B=1, HW=4, C=8, eps=1e-5), **change).items():
+            setattr(a, k, v)
+        return lib.cvb_residual_norm_fwd(ctypes.byref(a))
+
+    def bwd(**change):
+        a = _arguments()
+        for k, v in dict(dict(x=one, branch=one, dy=one, dx=one, B=1, HW=4, C=8, eps=1e-5), **change).items():
+            setattr(a, k, v)
+        return lib.cvb_residual_norm_bwd(ctypes.byref(a))
+
+    # addresses between elements
+    for name in ("x", "branch", "y"):
+        assert fwd(**{name: 18}) == -1 and fwd(**{name: 17, "io_dtype": 1}) == -1, name
+    for name in ("scale", "stats", "post_w"):
+        assert fwd(**{name: 18}) == -1, name
+    assert fwd(gate=18, gate_kind=1) == -1 and fwd(gate=18, gate_kind=2, io_dtype=1) == -1
+    assert fwd(post_w=one, post_b=18) == -1 and fwd(pre_w=18, z=one) == -1 and fwd(pre_w=one, z=18) == -1
+    for name in ("dy", "dx", "dbranch"):
+        assert bwd(**{name: 18}) == -1, name
+    assert bwd(dscale=18, workspace=one, workspace_bytes=1 << 30) == -1
+    assert bwd(dscale=one, workspace=18, workspace_bytes=1 << 30) == -4
+    assert bwd(gate=one, gate_kind=1, dgate=18) == -1 and bwd(gate=one, gate_kind=2, dgate=18, io_dtype=1) == -1
