@@ -786,7 +786,7 @@ size_t cvb_clip_workspace_bytes(int count) { return clip_workspace(count, sm_cou
 
 int cvb_clip_by_norm(const cvb_span* spans, int count, int kind, double max_norm, int scale_them, float* norm,
                      void* workspace, size_t workspace_bytes, void* stream) {
-  if (count < 0 || (count && !spans) || !norm || kind < 0 || kind > 2) return CVB_ERR_BAD_ARGUMENT;
+  if (count < 0 || (count && !spans) || !norm || !at_elements(sizeof(float), norm) || kind < 0 || kind > 2) return CVB_ERR_BAD_ARGUMENT;
   if (scale_them && !(max_norm >= 0)) return CVB_ERR_BAD_ARGUMENT;
   for (int i = 0; i < count; ++i) {
     const cvb_span& s = spans[i];
@@ -797,7 +797,8 @@ int cvb_clip_by_norm(const cvb_span* spans, int count, int kind, double max_norm
     if (s.n && (!s.out || (size_t)s.out % (s.out_type == CVB_F32 ? 4 : 2) || (s.in == s.out && s.in_type != s.out_type)))
       return CVB_ERR_BAD_ARGUMENT;
   }
-  if (!workspace || workspace_bytes < clip_workspace(count, sm_count())) return CVB_ERR_WORKSPACE;
+  if (!workspace || !at_elements(sizeof(double), workspace) || workspace_bytes < clip_workspace(count, sm_count()))
+    return CVB_ERR_WORKSPACE;
   return run_clip(spans, count, kind, max_norm, scale_them != 0, norm, workspace, sm_count(), (cudaStream_t)stream);
 }
 

@@ -375,7 +375,7 @@ int cvb_residual_norm_bwd(const cvb_residual_norm_args* args);
  * The norm of `count` tensors together (kind 1: sum of magnitudes, 2: Euclidean, 0: largest magnitude) and, with `scale_them`,
  * out = in . min(1, max_norm / (norm + 1e-6)) for each: what training does with its gradients before a step.
  *   spans : host array; in, out device pointers aligned to their elements; out may be in (same type) and overlaps nothing else
- *   norm  : device float
+ *   norm  : device float; workspace: at a boundary of 8 bytes
  * Sums in 64 bits, in an order of their own: equal calls give equal bits.  Infinities and NaN reach the norm; out is then what
  * the formula gives.  Where in is out and the norm is small enough, nothing is written to it.
  */

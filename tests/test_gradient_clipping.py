@@ -238,3 +238,15 @@ def test_c_abi_refusals():
     assert call(Span(16, 16, 4, 3, 0)) == -1
     assert call(kind=3) == call(count=-1) == call(norm=None) == call(max_norm=-1.0) == call(max_norm=float("nan")) == -1
     assert call(work=None) == call(size=ws - 1) == -4
+
+
+def test_c_abi_addresses():
+    from conversenet_b200 import _cabi
+    lib = _cabi.load()
+    p, size = ctypes.c_void_p(16), lib.cvb_clip_workspace_bytes(0)        # never dereferenced: validation fails first
+
+    def call(norm=p, work=p):
+        return lib.cvb_clip_by_norm(None, 0, 2, 1.0, 0, norm, work, size, None)
+
+    assert call(work=ctypes.c_void_p(20)) == -4                # sums of 64 bits
+    assert call(norm=ctypes.c_void_p(18)) == -1
