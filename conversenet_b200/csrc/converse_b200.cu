@@ -47,6 +47,8 @@ static const StaticEntry kStatic[] = {
 template <class... T>
 bool at_elements(size_t size, const T*... p) { return (((size_t)p % size == 0) && ...); }
 
+size_t io_size(int io_dtype) { return io_dtype == CVB_BF16 ? 2 : 4; }
+
 // Device word set by a kernel whose bounded wait gave up (one per device).
 __device__ int g_device_status;
 int* status_ptr() {
@@ -726,7 +728,7 @@ static int seam_params(const cvb_residual_norm_args& A, bool backward, seam::Par
   if (A.gate_kind < CVB_GATE_NONE || A.gate_kind > CVB_GATE_IMAGE || (A.gate_kind != CVB_GATE_NONE) != (A.gate != nullptr))
     return CVB_ERR_BAD_ARGUMENT;
   if ((A.post_b && !A.post_w) || (A.pre_b && !A.pre_w) || !(A.eps >= 0.f)) return CVB_ERR_BAD_ARGUMENT;
-  const size_t e = A.io_dtype == CVB_BF16 ? 2 : 4;
+  const size_t e = io_size(A.io_dtype);
   if (!at_elements(e, A.x, A.branch, A.y, A.z, A.dy, A.dz, A.dx, A.dbranch) ||
       !at_elements(A.gate_kind == CVB_GATE_FULL ? e : sizeof(float), A.gate, A.dgate) ||
       !at_elements(sizeof(float), A.scale, A.post_w, A.post_b, A.pre_w, A.pre_b, A.stats, A.dscale, A.dpost_w, A.dpost_b, A.dpre_w, A.dpre_b))
@@ -815,7 +817,8 @@ int cvb_quantize_tokens(const void* x, signed char* q, float* scale, long long B
                         int channels_last, int io_dtype, void* stream) {
   const int rc = check_int8(B, HW, K, io_dtype);
   if (rc != CVB_OK) return rc;
-  if (!x || !scale || !int8_rows(q, ldq, K)) return CVB_ERR_BAD_ARGUMENT;
+  if (!x || !scale || !int8_rows(q, ldq, K) || !at_elements(io_size(io_dtype), x) || !at_elements(sizeof(float), scale))
+    return CVB_ERR_BAD_ARGUMENT;
   return i8::run_quantize(x, q, scale, B, HW, K, ldq, int8_last(channels_last, HW), io_dtype, (cudaStream_t)stream);
 }
 
@@ -825,6 +828,7 @@ int cvb_int8_product(const signed char* q, long long ldq, const float* scale, co
   const int rc = check_int8(B, HW, K, io_dtype);
   if (rc != CVB_OK) return rc;
   if (!int8_rows(q, ldq, K) || !int8_rows(w, ldw, K) || !scale || !w_scale || !out || N < 1) return CVB_ERR_BAD_ARGUMENT;
+  if (!at_elements(sizeof(float), scale, w_scale, bias) || !at_elements(io_size(io_dtype), out)) return CVB_ERR_BAD_ARGUMENT;
   return i8::run_product(q, ldq, scale, w, ldw, w_scale, bias, out, B, HW, K, N, int8_last(channels_last, HW), io_dtype, sm_count(),
                          status_ptr(), (cudaStream_t)stream);
 }
@@ -840,6 +844,7 @@ int cvb_pointwise_int8(const void* x, const signed char* w, long long ldw, const
   const int rc = check_int8(B, HW, K, io_dtype);
   if (rc != CVB_OK) return rc;
   if (!x || !int8_rows(w, ldw, K) || !w_scale || !out || N < 1) return CVB_ERR_BAD_ARGUMENT;
+  if (!at_elements(io_size(io_dtype), x, out) || !at_elements(sizeof(float), w_scale, bias)) return CVB_ERR_BAD_ARGUMENT;
   const size_t need = i8::workspace(B, HW, K, N, int8_last(channels_last, HW), io_dtype, sm_count());
   if (need && (!workspace || (size_t)workspace % 16 || workspace_bytes < need)) return CVB_ERR_WORKSPACE;
   return i8::run_pointwise(x, w, ldw, w_scale, bias, out, B, HW, K, N, int8_last(channels_last, HW), io_dtype, workspace, sm_count(),

@@ -399,6 +399,7 @@ int cvb_clip_by_norm(const cvb_span* spans, int count, int kind, double max_norm
  *   cvb_int8_product    : q (B HW rows), w (N rows): rows of ldq and ldw bytes, multiples of 16, both addresses 16-byte aligned;
  *                         out channels_last 0: (B,N,HW); 1: (B,HW,N); bias (N) or NULL
  *   cvb_pointwise_int8  : the two together; the workspace holds q and the scales where they are not made on the way
+ * Every other address at a boundary of its elements (the workspace of 16 bytes).
  */
 int cvb_quantize_tokens(const void* x, signed char* q, float* scale, long long B, long long HW, int K, long long ldq,
                         int channels_last, int io_dtype, void* stream);

@@ -416,3 +416,23 @@ def test_planes_that_end_inside_a_warp(HW, K):
     qt, st = CF.quantize_tokens(x)
     for fmt in ("channels_first", "channels_last"):
         _check_product(CF.int8_product(qt, st, wq, ws, data_format=fmt), q, scale, wq, ws, None, fmt == "channels_first")
+
+
+def test_c_abi_addresses():
+    from conversenet_b200 import _cabi
+    lib = _cabi.load()
+    p = ctypes.c_void_p(16)                                # never dereferenced: validation fails first
+    f = lib.cvb_int8_product
+    # addresses between elements
+    assert lib.cvb_quantize_tokens(ctypes.c_void_p(18), p, p, 1, 4, 8, 16, 0, 0, None) == -1
+    assert lib.cvb_quantize_tokens(ctypes.c_void_p(17), p, p, 1, 4, 8, 16, 0, 1, None) == -1
+    between = ctypes.c_void_p(18)
+    assert lib.cvb_quantize_tokens(p, p, between, 1, 4, 8, 16, 0, 0, None) == -1
+    assert f(p, 16, between, p, 16, p, None, p, 1, 4, 8, 4, 0, 0, None) == -1
+    assert f(p, 16, p, p, 16, between, None, p, 1, 4, 8, 4, 0, 0, None) == -1
+    assert f(p, 16, p, p, 16, p, between, p, 1, 4, 8, 4, 0, 0, None) == -1
+    assert f(p, 16, p, p, 16, p, None, between, 1, 4, 8, 4, 0, 0, None) == -1
+    for change in (0, 3, 4, 5):
+        args = [p, p, 64, p, p, p]
+        args[change] = between
+        assert lib.cvb_pointwise_int8(*args, 1, 100, 64, 8, 0, 0, None, 0, None) == -1, change
