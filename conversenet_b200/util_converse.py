@@ -229,14 +229,22 @@ class ConverseBlock(nn.Module):
             return last[1]
         return self._pack.get(key, params, lambda: host.block_pack(*params))
 
+    @staticmethod
+    def _plain_layers(c1, c2):
+        """Whether the 1x1 layers have weights for the block's kernels to read (and are not, say, `Int8Pointwise`)."""
+        a, b, c, d = c1["1"], c1["5"], c2["1"], c2["3"]
+        if type(a) is type(b) is type(c) is type(d) is nn.Conv2d:
+            return True
+        return all(isinstance(getattr(m, "weight", None), torch.Tensor) for m in (a, b, c, d))
+
     def _forward_trainable(self, x, alpha1=None, alpha2=None):
         """The block under autograd through the native kernels; None where they do not apply (other widths, dtypes or
-        scales, hooked children, autocast, planes without a gradient kernel)."""
+        scales, other layers, hooked children, autocast, planes without a gradient kernel)."""
         c1, c2 = self.conv1._modules, self.conv2._modules
         conv = c1["3"]
         if not (BLOCK_FUSION and torch.is_grad_enabled() and x.is_cuda and x.dim() == 4 and x.size(1) == 64 and
-                x.dtype == torch.float32 and c1["1"].out_channels == 128 and c1["5"].out_channels == 64 and
-                conv.scale == 1 and not torch.is_autocast_enabled()):
+                x.dtype == torch.float32 and self._plain_layers(c1, c2) and c1["1"].out_channels == 128 and
+                c1["5"].out_channels == 64 and conv.scale == 1 and not torch.is_autocast_enabled()):
             return None
         params = CF.block_parameters(c1["0"], c1["1"], c1["5"], alpha1, c2["0"], c2["1"], c2["3"], alpha2)
         given = [q for i, q in enumerate(params) if i not in (6, 13)] + [conv.weight, conv.bias]
@@ -261,7 +269,7 @@ class ConverseBlock(nn.Module):
         if torch.is_grad_enabled() and (x.requires_grad or any(q.requires_grad for q in self.parameters())):
             return False  # the fused block kernels are forward-only
         c1, c2 = self.conv1._modules, self.conv2._modules
-        return (x.is_cuda and x.dim() == 4 and x.size(1) == 64 and c1["1"].out_channels == 128 and
+        return (x.is_cuda and x.dim() == 4 and x.size(1) == 64 and self._plain_layers(c1, c2) and c1["1"].out_channels == 128 and
                 c1["5"].out_channels == 64 and c1["3"].scale == 1 and x.dtype in (torch.float32, torch.bfloat16) and
                 c1["1"].bias is not None and c1["5"].bias is not None and c2["1"].bias is not None and
                 c2["3"].bias is not None and BLOCK_FUSION)

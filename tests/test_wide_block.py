@@ -124,3 +124,82 @@ def test_serving_in_integers(block):
         assert float((out - want).norm() / want.norm()) <= 1e-3
         # eight bits: every operand of four layers is off by at most half of 1/127 of its largest
         assert float((out - full).norm() / full.norm()) <= 0.05
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", [("conv1", 1), ("conv1", 5), ("conv2", 1), ("conv2", 3), None], ids=str)
+@pytest.mark.parametrize("alphas", [False, True])
+def test_integer_layers_in_the_64_channel_block(which, alphas):
+    """The framework's own blocks with one or all of their 1x1 layers replaced: every layer is called, as in a block of another width."""
+    from conversenet_b200 import ConverseBlock, ConverseBlockAlphaVariant
+    torch.manual_seed(0)
+    m = (ConverseBlockAlphaVariant if alphas else ConverseBlock)(64, 64, 3, padding=2).cuda().eval()
+    if alphas:
+        with torch.no_grad():
+            m.alpha1.normal_(), m.alpha2.normal_()
+    x = torch.randn(2, 64, 24, 20, device="cuda")
+    with torch.no_grad():
+        full = m(x)
+    for name, i in [which] if which else [("conv1", 1), ("conv1", 5), ("conv2", 1), ("conv2", 3)]:
+        getattr(m, name)[i] = Int8Pointwise(getattr(m, name)[i])
+
+    def layers(v):
+        a1, a2 = (m.alpha1, m.alpha2) if alphas else (1, 1)
+        v = a1 * m._branch1(v) + v
+        return a2 * m.conv2(v) + v
+
+    from conversenet_b200.util_converse import _exact_fp32
+    with torch.no_grad(), _exact_fp32():
+        want = layers(x)
+    with torch.no_grad():
+        out = m(x)
+        # eight bits: every operand of four layers is off by at most half of 1/127 of its largest
+        assert torch.equal(out, want) and 0 < float((out - full).norm() / full.norm()) <= 0.05
+    with pytest.raises(RuntimeError, match="inference"):
+        m(x)
+    for p in m.parameters():
+        p.requires_grad_(False)
+    assert torch.equal(m(x), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [None, torch.bfloat16])
+def test_integer_layers_in_the_denoiser(dtype):
+    from conversenet_b200 import ConverseBlock
+    from conversenet_b200.models import ConverseDnCNN
+    torch.manual_seed(0)
+    net = ConverseDnCNN().cuda().eval()
+    net.activation_dtype = dtype
+    x = torch.rand(1, 1, 24, 28, device="cuda")
+    with torch.no_grad():
+        for m in net.modules():
+            if isinstance(m, ConverseBlock):
+                for seq in (m.conv1, m.conv2):
+                    for i, layer in enumerate(seq):
+                        if isinstance(layer, nn.Conv2d):
+                            seq[i] = Int8Pointwise(layer)
+        out = net(x)
+        assert out.shape == x.shape and bool(torch.isfinite(out).all())
+        assert torch.equal(out, net(x))
+
+
+def test_which_layers_the_block_kernels_read():
+    from conversenet_b200 import ConverseBlock
+
+    class Shared(nn.Module):                       # a layer of someone's own around a convolution's weights
+        def __init__(self, conv):
+            super().__init__()
+            self.weight, self.bias, self.out_channels = conv.weight, conv.bias, conv.out_channels
+
+    m = ConverseBlock(64, 64)
+
+    def plain():
+        return m._plain_layers(m.conv1._modules, m.conv2._modules)
+
+    assert plain()
+    m.conv1[5] = Shared(m.conv1[5])
+    assert plain()
+    for seq, i in ((m.conv1, 1), (m.conv2, 3)):
+        kept, seq[i] = seq[i], nn.Identity()
+        assert not plain()
+        seq[i] = kept
