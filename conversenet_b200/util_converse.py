@@ -366,7 +366,8 @@ class ResidualNorm(nn.Module):
 class Int8Pointwise(nn.Module):
     """A 1x1 convolution or a linear layer in 8-bit integers, for inference (`functional.pointwise_int8`): weights as integers
     with a scale for each output channel, every token of the input quantised by its largest channel.  `layer` is on a CUDA
-    device; later changes of its weights do not reach the module."""
+    device; later changes of its weights do not reach the module.  Scales and biases stay in 32 bits whatever type the module is
+    cast to."""
 
     def __init__(self, layer):
         super().__init__()
@@ -385,6 +386,14 @@ class Int8Pointwise(nn.Module):
         self.register_buffer("weight_rows", rows)
         self.register_buffer("weight_scale", scale)
         self.register_buffer("bias", None if layer.bias is None else layer.bias.detach().float().clone())
+
+    def _apply(self, fn, recurse=True):
+        kept = {name: getattr(self, name) for name in ("weight_scale", "bias")}
+        super()._apply(fn, recurse)
+        for name, t in kept.items():
+            if t is not None and getattr(self, name).dtype != torch.float32:
+                setattr(self, name, t.to(getattr(self, name).device))
+        return self
 
     def forward(self, x):
         return CF.pointwise_int8(x, self.weight_rows[:, :self.in_channels], self.weight_scale, self.bias, self.data_format)

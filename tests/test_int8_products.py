@@ -436,3 +436,21 @@ def test_c_abi_addresses():
         args = [p, p, 64, p, p, p]
         args[change] = between
         assert lib.cvb_pointwise_int8(*args, 1, 100, 64, 8, 0, 0, None, 0, None) == -1, change
+
+
+@pytest.mark.gpu
+def test_a_module_of_another_type_keeps_its_scales():
+    """Casting the module leaves scales and biases in 32 bits: rounded to bf16 every output would be 2^-9 off."""
+    torch.manual_seed(1)
+    conv = torch.nn.Conv2d(64, 48, 1).cuda()
+    x = _features((1, 64, 9, 10), True, torch.float32, 6)
+    m = Int8Pointwise(conv)
+    y = m(x)
+    state = m.state_dict()
+    for cast in (torch.nn.Module.bfloat16, torch.nn.Module.half, torch.nn.Module.double, lambda n: n.cpu().to("cuda", torch.bfloat16)):
+        n = cast(torch.nn.Sequential(Int8Pointwise(conv)))
+        assert n[0].weight_scale.dtype == n[0].bias.dtype == torch.float32 and n[0].weight_scale.is_cuda
+        assert torch.equal(n(x), y)
+        n[0].load_state_dict(state)
+        assert torch.equal(n(x), y)
+    assert Int8Pointwise(torch.nn.Linear(64, 8, bias=False).cuda()).bfloat16().bias is None
