@@ -17,6 +17,11 @@ void floating(const at::Tensor& t, const char* what) {
   if (t.defined() && !t.is_floating_point()) throw Failed(std::string(what) + " must be a floating-point tensor");
 }
 
+// (the kernels would lose it)
+void no_tangent(const at::Tensor& t) {
+  if (t.defined() && t._fw_grad(0).defined()) throw Failed("this operator has no forward-mode derivative, and an input is a dual tensor");
+}
+
 // The residual seam's arguments, checked, and laid out for the kernels
 enum { kX, kBranch, kScale, kGate, kPostW, kPostB, kPreW, kPreB, kSeamTensors };
 struct SeamConfig {
@@ -193,6 +198,7 @@ PyObject* py_residual_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     static const char* names[] = {"x", "branch", "scale", "gate", "post_weight", "post_bias", "pre_weight", "pre_bias"};
     std::array<at::Tensor, kSeamTensors> t;
     for (int i = 0; i < kSeamTensors; ++i) t[i] = i <= kBranch ? cuda_tensor(a[i], names[i]) : optional(a[i], names[i]);
+    for (const at::Tensor& one : t) no_tangent(one);
     SeamConfig c;
     c.eps = real(a[8]);
     c.rms = PyObject_IsTrue(a[9]); c.sigmoid = PyObject_IsTrue(a[10]); c.last = PyObject_IsTrue(a[11]);
@@ -401,6 +407,8 @@ struct Int8Weight {
     N = (int)w.size(0);
     floating(scale, "weight_scale");
     floating(bias, "bias");
+    no_tangent(scale);
+    no_tangent(bias);
     if (scale.numel() != N) throw Failed("weight_scale must hold a value for each output channel");
     if (bias.defined() && bias.numel() != N) throw Failed("bias must hold a value for each output channel");
     same_device(w, x, "weight_q");
@@ -419,6 +427,7 @@ PyObject* py_quantize_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     want(n, 2);
     const at::Tensor& x0 = cuda_tensor(a[0], "x");
+    no_tangent(x0);
     const c10::cuda::CUDAGuard dev(x0.device());
     const int io = io_type(x0);
     const Tokens t(x0, PyObject_IsTrue(a[1]));
@@ -453,6 +462,7 @@ PyObject* py_int8_product(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Tokens t(q0, true);
     if (!last) t.B = q0.size(0), t.HW = q0.size(1) * q0.size(2), t.last = false;
     floating(s0, "scale");
+    no_tangent(s0);
     same_device(s0, q0, "scale");
     if (s0.numel() != t.B * t.HW) throw Failed("scale must hold a value for each token");
     Int8Weight w(a[2], a[3], a[4], q0, t.K);
@@ -479,6 +489,7 @@ PyObject* py_pointwise_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     want(n, 5);
     const at::Tensor& x0 = cuda_tensor(a[0], "x");
+    no_tangent(x0);
     const c10::cuda::CUDAGuard dev(x0.device());
     const int io = io_type(x0);
     const Tokens t(x0, PyObject_IsTrue(a[4]));

@@ -231,7 +231,8 @@ def residual_norm(x, branch, scale=None, gate=None, post_weight=None, post_bias=
     channels_last); `gate_act` is None or "sigmoid".  x and branch: (B,C,H,W), or (...,C) in channels_last, float32 or
     bfloat16, both of one type; strided tensors are copied.  z comes from y before it is rounded to that type.
 
-    Differentiable in every tensor (once).  Up to 16384 channels, with gradients in channels_first 4096."""
+    Differentiable in every tensor (once, and not in forward mode: dual tensors are refused).  Up to 16384 channels, with
+    gradients in channels_first 4096."""
     last = _channels_last(data_format)
     if norm not in ("layer", "rms"):
         raise ValueError("norm must be 'layer' | 'rms', got: %r" % (norm,))

@@ -454,3 +454,20 @@ def test_a_module_of_another_type_keeps_its_scales():
         n[0].load_state_dict(state)
         assert torch.equal(n(x), y)
     assert Int8Pointwise(torch.nn.Linear(64, 8, bias=False).cuda()).bfloat16().bias is None
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+    x = torch.randn(1, 16, 4, 4, device="cuda")
+    wq, ws = CF.quantize_weight(torch.randn(8, 16, device="cuda"))
+    bias = torch.randn(8, device="cuda")
+    q, s = CF.quantize_tokens(x)
+    with fwd.dual_level():
+        dual = [fwd.make_dual(v, torch.ones_like(v)) for v in (x, ws, bias, s)]
+        for call in (lambda: CF.pointwise_int8(dual[0], wq, ws, bias), lambda: CF.pointwise_int8(x, wq, dual[1], bias),
+                     lambda: CF.pointwise_int8(x, wq, ws, dual[2]), lambda: CF.quantize_tokens(dual[0]),
+                     lambda: CF.int8_product(q, dual[3], wq, ws), lambda: CF.int8_product(q, s, wq, dual[1]),
+                     lambda: CF.int8_product(q, s, wq, ws, dual[2])):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()

@@ -679,3 +679,19 @@ def test_c_abi_addresses():
     assert bwd(dscale=18, workspace=one, workspace_bytes=1 << 30) == -1
     assert bwd(dscale=one, workspace=18, workspace_bytes=1 << 30) == -4
     assert bwd(gate=one, gate_kind=1, dgate=18) == -1 and bwd(gate=one, gate_kind=2, dgate=18, io_dtype=1) == -1
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused():
+    """There is no tangent of the outputs: a call that would lose one says so."""
+    import torch.autograd.forward_ad as fwd
+    t = {n: v for n, v in _case("first", 8, 1, 4, 4, torch.float32, "layer", True, "full", True).items() if n in NAMES}
+    y0, z0 = _call(t, "first", "layer", True)
+    for leaf in (False, True):
+        with fwd.dual_level():
+            for n in t:
+                v = t[n].clone().requires_grad_(leaf)
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    _call(dict(t, **{n: fwd.make_dual(v, torch.ones_like(v))}), "first", "layer", True)
+            y, z = _call(t, "first", "layer", True)
+            assert torch.equal(y, y0) and torch.equal(z, z0)
