@@ -293,6 +293,9 @@ PyObject* py_clip_by_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!first.is_cuda()) throw Failed("the tensors must be CUDA tensors; this build has no CPU path");
     const c10::Device where = first.device();
     const c10::cuda::CUDAGuard dev(where);
+    // (gradients may have one, of a double backward: they are scaled in place all the same, as torch does it)
+    const bool history = !self && at::GradMode::is_enabled();
+    const char* no_history = "norms and scaled tensors have no history: call it under torch.no_grad() for tensors that require gradients";
     at::Tensor norm;
     std::vector<at::Tensor> made;          // new tensors
     {
@@ -309,6 +312,8 @@ PyObject* py_clip_by_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         };
         const c10::TensorImpl* impl = t.unsafeGetTensorImpl();
         if (impl->layout() != at::kStrided) throw Failed("sparse tensors are not supported");
+        if (history && t.requires_grad()) throw Failed(no_history);
+        no_tangent(t);
         if (impl->device() != where) throw Failed("the tensors must be on one CUDA device; this build has no CPU path");
         s[i].in_type = s[i].out_type = io_type(t);
         s[i].n = impl->numel();
@@ -321,6 +326,7 @@ PyObject* py_clip_by_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
           const c10::TensorImpl* to = o.unsafeGetTensorImpl();
           if (to->layout() != at::kStrided || to->sizes() != impl->sizes()) throw Failed("each tensor of out must have the shape of its tensor");
           if (to->device() != where) throw Failed("out must be on the device of the tensors");
+          if (history && !fresh && o.requires_grad()) throw Failed(no_history);
           s[i].out_type = io_type(o);
           if (!(whole && to->is_contiguous()) && !(flat && o.strides() == t.strides())) {
             if (!to->is_contiguous()) throw Failed("a tensor of out must be contiguous or have the strides of its tensor");

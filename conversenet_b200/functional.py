@@ -255,14 +255,15 @@ def _norm_kind(norm_type):
 
 
 def grad_norm(tensors, norm_type=2.0):
-    """The norm of all tensors together, a float32 tensor on their device (sums in 64 bits; the same bits at every call)."""
+    """The norm of all tensors together, a float32 tensor on their device (sums in 64 bits; the same bits at every call).  Not
+    differentiable: tensors that require gradients are refused outside torch.no_grad()."""
     return _clip_norm(tensors, False, norm_type, 0.0)[1]
 
 
 def clip_by_global_norm(tensors, max_norm, norm_type=2.0, out=None):
     """(the tensors times min(1, max_norm / (norm + 1e-6)), norm): `grad_norm`'s norm, and the tensors scaled so that it does
     not exceed `max_norm`.  `out`: tensors of the same shapes, float32 or bfloat16 whatever the inputs are (master gradients
-    in 32 bits), that receive them; they may be the tensors themselves.  Not differentiable."""
+    in 32 bits), that receive them; they may be the tensors themselves.  Not differentiable: as `grad_norm`."""
     return _clip_norm(tensors, out, norm_type, max_norm)
 
 
@@ -272,8 +273,11 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     grads = [p.grad for p in parameters if p.grad is not None]
-    if error_if_nonfinite and not bool(torch.isfinite(grad_norm(grads, norm_type))):
-        raise RuntimeError("The total norm of order %s for gradients is not finite, so they cannot be clipped" % norm_type)
+    if error_if_nonfinite:
+        with torch.no_grad():
+            finite = bool(torch.isfinite(grad_norm(grads, norm_type)))
+        if not finite:
+            raise RuntimeError("The total norm of order %s for gradients is not finite, so they cannot be clipped" % norm_type)
     return _clip_norm(grads, True, norm_type, max_norm)[1]
 
 

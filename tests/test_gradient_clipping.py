@@ -250,3 +250,32 @@ def test_c_abi_addresses():
 
     assert call(work=ctypes.c_void_p(20)) == -4                # sums of 64 bits
     assert call(norm=ctypes.c_void_p(18)) == -1
+
+
+@pytest.mark.gpu
+def test_tensors_with_a_history():
+    """No result has one: where one would be recorded the call is refused; `clip_grad_norm_` records none, as torch's own does not."""
+    import torch.autograd.forward_ad as fwd
+    p = torch.nn.Parameter(torch.randn(50, device="cuda"))
+    x = torch.randn(50, device="cuda")
+    loss = (p ** 3).sum()
+    grad, = torch.autograd.grad(loss, p, create_graph=True)
+    assert grad.requires_grad
+    for call in (lambda: CF.grad_norm([x, grad]), lambda: CF.grad_norm([p]), lambda: CF.clip_by_global_norm([grad], 1.0),
+                 lambda: CF.clip_by_global_norm([x], 1.0, out=[p]), lambda: CF.clip_by_global_norm([x], 1.0, out=[p * 1])):
+        with pytest.raises(RuntimeError, match="no_grad"):
+            call()
+    with torch.no_grad():
+        assert float(CF.grad_norm([grad])) == pytest.approx(float(grad.norm()), rel=1e-5)
+        out, _ = CF.clip_by_global_norm([grad], 1.0)
+        CF.clip_by_global_norm([x], 1.0, out=[p])
+    assert not out[0].requires_grad and float(p.norm()) == pytest.approx(1.0, rel=1e-5)
+    p.grad = grad
+    before = float(grad.norm())
+    assert float(CF.clip_grad_norm_([p], 0.5 * before, error_if_nonfinite=True)) == pytest.approx(before, rel=1e-5)
+    assert float(p.grad.norm()) == pytest.approx(0.5 * before, rel=1e-5)
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, torch.ones_like(x))
+        for call in (lambda: CF.grad_norm([dual]), lambda: CF.clip_by_global_norm([dual], 1.0)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
