@@ -264,6 +264,11 @@ def clip_by_global_norm(tensors, max_norm, norm_type=2.0, out=None):
     """(the tensors times min(1, max_norm / (norm + 1e-6)), norm): `grad_norm`'s norm, and the tensors scaled so that it does
     not exceed `max_norm`.  `out`: tensors of the same shapes, float32 or bfloat16 whatever the inputs are (master gradients
     in 32 bits), that receive them; they may be the tensors themselves.  Not differentiable: as `grad_norm`."""
+    if out is not None:
+        tensors = tensors if isinstance(tensors, (list, tuple)) else list(tensors)
+        out = tensors if out is True else out if isinstance(out, (list, tuple)) else list(out)
+        if not tensors and len(out):
+            raise RuntimeError("out must hold a tensor for each of the tensors")
     return _clip_norm(tensors, out, norm_type, max_norm)
 
 

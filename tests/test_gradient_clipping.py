@@ -279,3 +279,17 @@ def test_tensors_with_a_history():
         for call in (lambda: CF.grad_norm([dual]), lambda: CF.clip_by_global_norm([dual], 1.0)):
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
+
+
+@pytest.mark.gpu
+def test_outputs_from_any_iterable():
+    x = [torch.randn(9, device="cuda"), torch.randn(5, device="cuda")]
+    into = [torch.empty_like(t) for t in x]
+    out, norm = CF.clip_by_global_norm(iter(x), 0.5, out=iter(into))
+    assert [a is b for a, b in zip(out, into)] == [True, True]
+    _check(into, x, float(norm), 0.5)
+    with pytest.raises(RuntimeError):
+        CF.clip_by_global_norm([], 0.5, out=into)
+    assert CF.clip_by_global_norm([], 0.5, out=[])[0] == []
+    with pytest.raises(TypeError):
+        CF.clip_by_global_norm(x, 0.5, out=False)
