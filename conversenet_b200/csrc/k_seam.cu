@@ -111,13 +111,58 @@ __device__ __forceinline__ void copy_pieces(void* to, const void* from, int byte
 }
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-// The gate's factor.  ex2.approx and the approximate reciprocal are good to 2 units in the last place; the product before them
-// loses |g| . 2^-24, so a sigmoid is off by 1e-6 of itself at |g| = 10.
-__device__ __forceinline__ float gate_of(float g, int act) { return act ? __fdividef(1.f, 1.f + __expf(-g)) : g; }
-// the same for a gate of an image, of which there are few: to the last place
+// A gate of each element: its sigmoid s = 1 / (1 + e), e = exp(-g) = 2^(-g log2 e).  fp32: with what the product and the constant lose,
+// which would be |g| 2^-24 of e (g kept where that is a number; NaN stays); ex2.approx is good to 2^-22, the reciprocal to a unit.
+// bf16: without, 1e-6 of s at |g| = 10 or a thousandth of the type's rounding.  Neither keeps numbers below 2^-126.
+// (expf and a division took 4 to 12 % more of the fp32 kernels' times forward and 5 to 26 % of the gradients'; this takes 0 to 3 and 0 to
+// 5 % more than s from __expf and s (1 - s) did, 8 x 96 x 128 x 128 fp32 gradients 118 -> 124 us the most.)
+template <typename IO>
+__device__ __forceinline__ float gate_exp(float g) {
+  const float log2e = 1.4426950216293335f, rest = 1.9259629911266175e-8f, ln2 = 0.6931471805599453f;
+  float e;
+  if (sizeof(IO) == 2) {
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -log2e));
+    return e;
+  }
+  asm("min.NaN.f32 %0, %0, 0f42D00000;" : "+f"(g));          // 104
+  asm("max.NaN.f32 %0, %0, 0fC2B00000;" : "+f"(g));          // -88
+  const float h = g * -log2e, c = fmaf(g, -rest, fmaf(g, -log2e, -h));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(h));
+  return fmaf(e * c, ln2, e);
+}
+__device__ __forceinline__ float reciprocal(float v) {
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(v));
+  return v;
+}
+// For the gradient it is held as the smaller of s and 1 - s, negative where it is 1 - s: so the slope s (1 - s) keeps all its digits (s
+// by itself has none of 1 - s from g = 17 on).  sigmoid_hold gives s and leaves that in g; gate_factor gives s from it, but for the last
+// place the same (`one`: the bits of 1, or 0 where the gate is taken as it is; -0 gives 1).  A forward kernel takes s the way that the
+// gradients' does.
+template <typename IO>
+__device__ __forceinline__ float sigmoid_hold(float& g) {
+  const float e = gate_exp<IO>(g), s = reciprocal(1.f + e);
+  g = g > 0.f ? -(e * s) : s;
+  return s;
+}
+__device__ __forceinline__ float gate_factor(float f, int one) { return f + __int_as_float((__float_as_int(f) >> 31) & one); }
+__device__ __forceinline__ float gate_slope(float f, bool act) { return act ? fmaf(-fabsf(f), fabsf(f), fabsf(f)) : 1.f; }
+constexpr int kOne = 0x3f800000;
+// channels_first
+template <typename IO>
+__device__ __forceinline__ float cf_gate_of(float g, int act) { return act ? reciprocal(1.f + gate_exp<IO>(g)) : g; }
+// channels_last
+template <typename IO>
+__device__ __forceinline__ float cl_gate_of(float g, int act) {
+  if (!act) return g;
+  sigmoid_hold<IO>(g);
+  return gate_factor(g, kOne);
+}
+// the gate of an image, of which there are few: to the last place
 __device__ __forceinline__ float image_gate_of(float g, int act) { return act ? 1.f / (1.f + expf(-g)) : g; }
-// its derivative, from the factor
-__device__ __forceinline__ float gate_slope(float s, int act) { return act ? s * (1.f - s) : 1.f; }
+__device__ __forceinline__ float image_gate_slope(float g, int act) {
+  const float e = expf(-fabsf(g)), s = 1.f / (1.f + e);
+  return act ? s * (e * s) : 1.f;
+}
 
 // ------------------------------------------------------------------ channels_first, forward
 // The VEC pixels of a thread: neighbours, read and written as vectors (ALONG), where rows are aligned to them; else 32 apart.
@@ -344,7 +389,7 @@ __global__ void __launch_bounds__(MAXT, MINB) cf_fwd_kernel(const __grid_constan
       float g[VEC];
       px.template load<IO>(P.gate, base + i * P.HW, g, i < n);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) v[i][j] = fmaf(fmaf(v[i][j], w[i & 3], o[i & 3]), gate_of(g[j], P.act), x[i][j]);
+      for (int j = 0; j < VEC; ++j) v[i][j] = fmaf(fmaf(v[i][j], w[i & 3], o[i & 3]), cf_gate_of<IO>(g[j], P.act), x[i][j]);
     } else {
 #pragma unroll
       for (int j = 0; j < VEC; ++j) v[i][j] = fmaf(v[i][j], w[i & 3], x[i][j] + o[i & 3]);
@@ -384,7 +429,7 @@ __device__ __forceinline__ float cf_sum_value(const Params& P, long long at, int
   if (P.gate_kind == kGateImage) a *= image_gate_of(((const float*)P.gate)[b * P.C + c], P.act);
   if (P.gate_kind == kGateFull) {
     Vec<IO, 1>::load(P.gate, at, &g);
-    v *= gate_of(g, P.act);
+    v *= cf_gate_of<IO>(g, P.act);
   }
   return fmaf(v, a, x);
 }
@@ -501,7 +546,8 @@ __global__ void __launch_bounds__(MAXT, MINB) cf_bwd_kernel(const __grid_constan
   float sa[CPT], sb[CPT], sw[CPT], so[CPT];       // sums A, B; dz k, dz
 #pragma unroll
   for (int i = 0; i < CPT; ++i) sa[i] = sb[i] = sw[i] = so[i] = 0.f;
-  const bool image = P.gate_kind == kGateImage;
+  const bool image = P.gate_kind == kGateImage, act = GATED && P.act;
+  const int one = act ? kOne : 0;
   const unsigned of = image ? blockIdx.x / P.parts : 0, first = of * P.tiles, last = image ? first + P.tiles : (unsigned)(P.tiles * P.B);
   for (int c = threadIdx.x; c < padded; c += blockDim.x) {
     const float2 f = branch_factors(P, c, of);
@@ -561,11 +607,7 @@ __global__ void __launch_bounds__(MAXT, MINB) cf_bwd_kernel(const __grid_constan
       get(px, 0, i, P.dz, row + i * P.HW, d[i]);
       get(px, 1, i, P.dz ? P.x : nullptr, row + i * P.HW, k[i]);
       get(px, 2, i, P.branch, row + i * P.HW, h[i]);
-      if constexpr (GATED) {
-        get(px, 3, i, P.gate, row + i * P.HW, f[i]);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) f[i][j] = gate_of(f[i][j], P.act);
-      }
+      if constexpr (GATED) get(px, 3, i, P.gate, row + i * P.HW, f[i]);
     }
     float mk[VEC], rk[VEC];
     if (P.dz) {
@@ -588,9 +630,10 @@ __global__ void __launch_bounds__(MAXT, MINB) cf_bwd_kernel(const __grid_constan
       for (int i = 0; i < CPT; ++i) {
         if (i % 4 == 0) four_of(wy + c0 + i, vec), four_of(oy + c0 + i, add);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)          // y again, as it was before it was rounded
-          k[i][j] = (GATED ? fmaf(fmaf(h[i][j], vec[i & 3], add[i & 3]), f[GATED ? i : 0][j], k[i][j])
-                           : fmaf(h[i][j], vec[i & 3], k[i][j] + add[i & 3])) - mk[j];
+        for (int j = 0; j < VEC; ++j) {        // y again, as it was before it was rounded
+          if constexpr (GATED) k[i][j] = fmaf(fmaf(h[i][j], vec[i & 3], add[i & 3]), act ? sigmoid_hold<IO>(f[i][j]) : f[i][j], k[i][j]) - mk[j];
+          else k[i][j] = fmaf(h[i][j], vec[i & 3], k[i][j] + add[i & 3]) - mk[j];
+        }
       }
 #pragma unroll
       for (int j = 0; j < VEC; ++j) u[j] = w[j] = 0.f;
@@ -617,6 +660,11 @@ __global__ void __launch_bounds__(MAXT, MINB) cf_bwd_kernel(const __grid_constan
       for (int i = 0; i < CPT; ++i)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) d[i][j] = rk[j] * (d[i][j] - fmaf(k[i][j], w[j], u[j]));
+    } else if (GATED && act) {
+#pragma unroll
+      for (int i = 0; i < CPT; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) sigmoid_hold<IO>(f[GATED ? i : 0][j]);
     }
 #pragma unroll
     for (int i = 0; i < CPT; ++i) {
@@ -642,11 +690,11 @@ __global__ void __launch_bounds__(MAXT, MINB) cf_bwd_kernel(const __grid_constan
         if (i < n && P.dgate) {
           float dg[VEC];
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) dg[j] = d[i][j] * fmaf(h[i][j], vec[i & 3], add[i & 3]) * gate_slope(f[i][j], P.act);
+          for (int j = 0; j < VEC; ++j) dg[j] = d[i][j] * fmaf(h[i][j], vec[i & 3], add[i & 3]) * gate_slope(f[i][j], act);
           px.template store<IO>(P.dgate, base + i * P.HW, dg);
         }
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) d[i][j] *= f[i][j];
+        for (int j = 0; j < VEC; ++j) d[i][j] *= gate_factor(f[i][j], one);
       }
     }
 #pragma unroll
@@ -760,10 +808,11 @@ __global__ void __launch_bounds__(1024) cf_bwd_wide_kernel(const __grid_constant
       h = (h - mh) * rh;
       if (P.gate_kind == kGateFull) {
         Vec<IO, 1>::load(P.gate, base + c * P.HW, &g);
-        g = gate_of(g, P.act);
+        float held = g;
+        if (P.act) g = sigmoid_hold<IO>(held);
         if (live && P.dgate) {
           const float pw = P.post_w ? P.post_w[c] : 1.f, pb = P.post_b ? P.post_b[c] : 0.f;
-          const float dg = d * (P.scale ? P.scale[c] : 1.f) * fmaf(h, pw, pb) * gate_slope(g, P.act);
+          const float dg = d * (P.scale ? P.scale[c] : 1.f) * fmaf(h, pw, pb) * gate_slope(held, P.act);
           Vec<IO, 1>::store(P.dgate, base + c * P.HW, &dg);
         }
       }
@@ -783,7 +832,7 @@ __global__ void __launch_bounds__(1024) cf_bwd_wide_kernel(const __grid_constant
       float g = 1.f, h;
       if (P.gate_kind == kGateFull) {
         Vec<IO, 1>::load(P.gate, base + c * P.HW, &g);
-        g = gate_of(g, P.act);
+        g = cf_gate_of<IO>(g, P.act);
       }
       float t = total(c) * factor(c, g);
       if (P.post_w) {
@@ -941,7 +990,7 @@ __global__ void __launch_bounds__(MAXT, MINB) cl_fwd_kernel(const __grid_constan
           if (P.gate_kind == kGateFull) {
             Vec<IO, V>::load(P.gate, base + c, g);
 #pragma unroll
-            for (int j = 0; j < V; ++j) g[j] = gate_of(g[j], P.act);
+            for (int j = 0; j < V; ++j) g[j] = cl_gate_of<IO>(g[j], P.act);
           }
 #pragma unroll
           for (int j = 0; j < V; ++j) y[i][j] = fmaf(fmaf((v[i][j] - mean) * rstd, wy[i][j], oy[i][j]), g[j], x[i][j]);
@@ -985,6 +1034,8 @@ __global__ void __launch_bounds__(MAXT, MINB) cl_bwd_kernel(const __grid_constan
   const int tpr = P.tpr, t = threadIdx.x & (tpr - 1), rows = blockDim.x / tpr, row = threadIdx.x / tpr;
   const float inv = 1.f / (float)P.C;
   const bool image = P.gate_kind == kGateImage;
+  const bool act = P.gate_kind == kGateFull && P.act;
+  const int one = act ? kOne : 0;
   const long long of = blockIdx.x / P.parts, first = image ? of * P.HW : 0, last = image ? first + P.HW : P.tokens;
   float sa[NV][V], sb[NV][V], sw[NV][V], so[NV][V], wy[NV][V], oy[NV][V], pw[NV][V];
 #pragma unroll
@@ -1056,19 +1107,32 @@ __global__ void __launch_bounds__(MAXT, MINB) cl_bwd_kernel(const __grid_constan
       for (int j = 0; j < V; ++j) h[i][j] = on ? (h[i][j] - mean) * rstd : 0.f, f[i][j] = 1.f;
       if (P.gate_kind == kGateFull) {
         get(3, i, P.gate, base + c, on, f[i]);
+        if (act) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) f[i][j] = gate_of(f[i][j], P.act);
+          for (int j = 0; j < V; ++j) sigmoid_hold<IO>(f[i][j]);
+        }
       }
     }
     begin(token + step);
     if (P.dz) {
       float u[2] = {0.f, 0.f};
+      // y again, as it was before it was rounded
+      if (act) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int j = 0; j < V; ++j) k[i][j] = fmaf(fmaf(h[i][j], wy[i][j], oy[i][j]), gate_factor(f[i][j], one), k[i][j]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+          for (int j = 0; j < V; ++j) k[i][j] = fmaf(fmaf(h[i][j], wy[i][j], oy[i][j]), f[i][j], k[i][j]);
+      }
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int j = 0; j < V; ++j) {          // (dz is 0 behind the last token and channel, and so are the sums)
-          // y again, as it was before it was rounded
-          k[i][j] = (fmaf(fmaf(h[i][j], wy[i][j], oy[i][j]), f[i][j], k[i][j]) - mk) * rk;
+          k[i][j] = (k[i][j] - mk) * rk;
           so[i][j] += d[i][j];
           sw[i][j] = fmaf(d[i][j], k[i][j], sw[i][j]);
           d[i][j] *= pw[i][j];
@@ -1096,11 +1160,11 @@ __global__ void __launch_bounds__(MAXT, MINB) cl_bwd_kernel(const __grid_constan
         if (P.dgate) {
           float o[V];
 #pragma unroll
-          for (int j = 0; j < V; ++j) o[j] = d[i][j] * fmaf(h[i][j], wy[i][j], oy[i][j]) * gate_slope(f[i][j], P.act);
+          for (int j = 0; j < V; ++j) o[j] = d[i][j] * fmaf(h[i][j], wy[i][j], oy[i][j]) * gate_slope(f[i][j], act);
           Vec<IO, V>::store(P.dgate, base + c, o);
         }
 #pragma unroll
-        for (int j = 0; j < V; ++j) d[i][j] *= f[i][j];
+        for (int j = 0; j < V; ++j) d[i][j] *= gate_factor(f[i][j], one);
       }
 #pragma unroll
       for (int j = 0; j < V; ++j) {          // (an image's sums are without its gate, which is in wy)
@@ -1199,8 +1263,8 @@ __global__ void __launch_bounds__(1024) finish_kernel(const __grid_constant__ Pa
       if (s % share) u0 = u1 = 0;
     }
     if (P.gate_kind == kGateImage && !pre && c < P.C && b < images && s % share == 0) {
-      const float g = image_gate_of(((const float*)P.gate)[(long long)b * P.C + c], P.act);
-      if (P.dgate) ((float*)P.dgate)[(long long)b * P.C + c] = (float)(a * (w * u0 + o * u1) * gate_slope(g, P.act));
+      const float held = ((const float*)P.gate)[(long long)b * P.C + c], g = image_gate_of(held, P.act);
+      if (P.dgate) ((float*)P.dgate)[(long long)b * P.C + c] = (float)(a * (w * u0 + o * u1) * image_gate_slope(held, P.act));
       u0 *= g;
       u1 *= g;
     }

@@ -695,3 +695,60 @@ def test_forward_mode_is_refused():
                     _call(dict(t, **{n: fwd.make_dual(v, torch.ones_like(v))}), "first", "layer", True)
             y, z = _call(t, "first", "layer", True)
             assert torch.equal(y, y0) and torch.equal(z, z0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout,C", [("first", 8), ("first", 300), ("last", 8), ("last", 7)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["full", "image"])
+def test_the_sigmoid_and_its_slope(layout, C, dtype, kind):
+    """From one end of the gate's range to the other.  u = 2^-24: e = exp(-g) is off by 2^-22 (ex2.approx) and two products' roundings, 6 u;
+    s = 1 / (1 + e) by that, a sum and an approximate quotient (2 units, 2^-22): 11 u; the smaller of s and 1 - s by one product more,
+    12 u; the slope is its product with one minus it: 14 u.  All is multiplied by 1 and added to 0.  A gate of an image is done with expf (2
+    units) and a division, which is less.  For a gate of each element in bf16 the exponent's argument is rounded too, |g| 2^-23 of e:
+    2^-17 at 2^6."""
+    first, T = layout == "first", 512 if kind == "full" else 1
+    B = 512 // T
+    g = torch.linspace(-64, 64, 512 * C, dtype=torch.float64, device="cuda")
+    g = g[torch.randperm(512 * C, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")].view(512, C)
+    g[0, 0], g[1, 0], g[2, 0], g[3, 0] = float("inf"), -float("inf"), torch.finfo(dtype).max, torch.finfo(dtype).min
+
+    def lay(v):
+        v = v.view(B, T, C)
+        return v.permute(0, 2, 1).reshape(B, C, T, 1).contiguous() if first else v
+
+    gate = lay(g.to(dtype)).requires_grad_(True)
+    x, branch = torch.zeros(gate.shape, dtype=dtype, device="cuda"), torch.ones(gate.shape, dtype=dtype, device="cuda")
+    if kind == "image":          # two pixels, so that it is one
+        x, branch = (v.repeat(1, 1, 2, 1) if first else v.repeat(1, 2, 1) for v in (x, branch))
+    branch.requires_grad_(True)
+    y = CF.residual_norm(x, branch, gate=gate, gate_act="sigmoid", data_format="channels_" + layout)
+    slope, through = torch.autograd.grad(y, (gate, branch), torch.ones_like(y))
+    exact = gate.detach().double()
+    e = torch.exp(-exact.abs())
+    small, large = e / (1 + e), 1 / (1 + e)
+    s, ds = torch.where(exact > 0, large, small).expand_as(y), small * large * (y.numel() // gate.numel())
+    last = torch.finfo(dtype).eps / 2
+    exactly = dtype == torch.float32 or kind == "image"
+    for got, want, tol in ((y.detach().double(), s, 11 * 2.0 ** -24 if exactly else 2.0 ** -16),
+                           (through.double(), s, 13 * 2.0 ** -24 if exactly else 2.0 ** -16),
+                           (slope.double(), ds, 14 * 2.0 ** -24 if exactly else 2.0 ** -15)):
+        over = (got - want).abs() - (tol + last) * want - 2.0 ** -126           # (numbers that fp32 flushes or loses digits of)
+        assert float(over.max()) <= 0, float((over / want.clamp(min=2.0 ** -126)).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["first", "last"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("gate", ["none", "full", "image"])
+def test_a_token_of_one_channel_has_no_spread(layout, dtype, gate):
+    """Its mean is itself: z is the bias, and nothing comes back through the norm.  The gradients' kernel forms y again, in every gate's
+    way to the last bit, or its difference from the mean would be 300 times larger than a rounding."""
+    t = _case(layout, 1, 2, 61, 47, dtype, "layer", False, gate, True)
+    names = [n for n in NAMES if n in t]
+    for n in names:
+        t[n].requires_grad_(True)
+    y, z = _call(t, layout, "layer", gate != "none")
+    got = dict(zip(names, torch.autograd.grad((y, z), [t[n] for n in names], (t["dy"], t["dz"]))))
+    assert torch.equal(z, t["pre_bias"].detach().to(dtype).expand_as(z))
+    assert torch.equal(got["x"], t["dy"]) and float(got["pre_weight"]) == 0
