@@ -112,13 +112,15 @@ __device__ __forceinline__ void copy_pieces(void* to, const void* from, int byte
 __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // A gate of each element: its sigmoid s = 1 / (1 + e), e = exp(-g) = 2^(-g log2 e).  fp32: with what the product and the constant lose,
-// which would be |g| 2^-24 of e (g kept where that is a number; NaN stays); ex2.approx is good to 2^-22, the reciprocal to a unit.
+// which would be |g| 2^-24 of e: the product's rounding error is itself an fma, and 2^(h + c) = 2^h (1 + c ln 2) for so small a c (g kept
+// where that is a number; NaN stays).  ex2.approx is good to 2^-22, the reciprocal to a unit.
 // bf16: without, 1e-6 of s at |g| = 10 or a thousandth of the type's rounding.  Neither keeps numbers below 2^-126.
 // (expf and a division took 4 to 12 % more of the fp32 kernels' times forward and 5 to 26 % of the gradients'; this takes 0 to 3 and 0 to
 // 5 % more than s from __expf and s (1 - s) did, 8 x 96 x 128 x 128 fp32 gradients 118 -> 124 us the most.)
 template <typename IO>
 __device__ __forceinline__ float gate_exp(float g) {
-  const float log2e = 1.4426950216293335f, rest = 1.9259629911266175e-8f, ln2 = 0.6931471805599453f;
+  constexpr double kLn2 = 0.693147180559945309417;
+  constexpr float log2e = (float)(1 / kLn2), rest = (float)(1 / kLn2 - (double)log2e), ln2 = (float)kLn2;
   float e;
   if (sizeof(IO) == 2) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -log2e));
