@@ -752,3 +752,37 @@ def test_a_token_of_one_channel_has_no_spread(layout, dtype, gate):
     got = dict(zip(names, torch.autograd.grad((y, z), [t[n] for n in names], (t["dy"], t["dz"]))))
     assert torch.equal(z, t["pre_bias"].detach().to(dtype).expand_as(z))
     assert torch.equal(got["x"], t["dy"]) and float(got["pre_weight"]) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [
+    ("first", 64, 1, 128, 96, "fp32", "layer", True, "full", True),
+    ("first", 300, 2, 9, 11, "fp32", "layer", True, "full", True),
+    ("first", 96, 2, 15, 17, "bf16", "rms", False, "image", True),
+    ("first", 1030, 1, 5, 7, "bf16", "layer", True, "image", False),
+    ("last", 64, 2, 24, 20, "bf16", "layer", True, "full", True),
+    ("last", 257, 3, 31, 3, "fp32", "layer", False, "full", False),
+    ("last", 1024, 2, 31, 3, "fp32", "rms", True, "image", True),
+], ids=lambda c: "-".join(map(str, c)))
+def test_a_gate_that_is_taken_as_it_is(case):
+    """gate_act None: against the formula, forward and gradients."""
+    layout, C, B, H, W, dtype, norm, post, gate, scale = case
+    t = _case(layout, C, B, H, W, {"fp32": torch.float32, "bf16": torch.bfloat16}[dtype], norm, post, gate, scale, seed=4)
+    names = [n for n in NAMES if n in t]
+    d = {n: v.double() for n, v in t.items()}
+    for n in names:
+        t[n].requires_grad_(True)
+        d[n].requires_grad_(True)
+    out, ref = _call(t, layout, norm, False), _formula(d, layout, norm, False)
+    dim = 1 if layout == "first" else -1
+    for a, b in zip(out, ref):
+        _close(a, b, dim, "outputs")
+    tops = _before_cancelling(d, layout, norm, False)
+    got = torch.autograd.grad(out, [t[n] for n in names], (t["dy"], t["dz"]))
+    want = torch.autograd.grad(ref, [d[n] for n in names], (d["dy"], d["dz"]))
+    for n, a, b in zip(names, got, want):
+        if n in ("x", "branch") or (n == "gate" and gate == "full"):
+            _close(a, b, dim, n, tops[n])
+        else:
+            # sums over tokens of terms of both signs: 1e-5 of the norm, as the parts above are held to, and the type's rounding
+            assert float((a.double() - b).norm()) <= (1e-5 + torch.finfo(a.dtype).eps / 2) * float(b.norm()), n
