@@ -394,7 +394,7 @@ int cvb_clip_by_norm(const cvb_span* spans, int count, int kind, double max_norm
  *     scale_t = max_k |x_tk| / 127,   q_tk = the integer nearest to x_tk / scale_t (an even one where two are as near),
  * decided exactly; weights are integers with a scale for each output channel, and
  *     out_tn = (sum_k q_tk w_nk) . scale_t . w_scale_n + bias_n,
- * the sum exact in 32-bit integers (K up to 131072).  A token with an infinity or a NaN gets the scale NaN, and so NaN outputs.
+ * the sum exact (K up to 131072; of any int8 values).  A token with an infinity or a NaN gets the scale NaN, and so NaN outputs.
  *   cvb_quantize_tokens : x channels_last 0: (B,K,HW); 1: (B,HW,K), contiguous, io_dtype -> q (B HW rows of ldq bytes), scale
  *   cvb_int8_product    : q (B HW rows), w (N rows): rows of ldq and ldw bytes, multiples of 16, both addresses 16-byte aligned;
  *                         out channels_last 0: (B,N,HW); 1: (B,HW,N); bias (N) or NULL
