@@ -228,8 +228,9 @@ def residual_norm(x, branch, scale=None, gate=None, post_weight=None, post_bias=
     mean square), with `post_weight` / `pre_weight` and optional biases.  Without `post_weight` the branch is taken as it is;
     without `pre_weight` the result is y, else (y, z).  `scale` holds a value for each channel (the alphas of
     `ConverseBlockAlphaVariant`), `gate` one for each element (of the type of x) or for each image and channel ((B,C,1,1),
-    or (B,1,...,C) in channels_last, of any floating type); `gate_act` is None (the gate as it is) or "sigmoid".  x and branch: (B,C,H,W), or (...,C) in channels_last, float32 or
-    bfloat16, both of one type; strided tensors are copied.  z comes from y before it is rounded to that type.
+    or (B,1,...,C) in channels_last, of any floating type); `gate_act` is None (the gate as it is) or "sigmoid".  x and
+    branch: (B,C,H,W), or (...,C) in channels_last, float32 or bfloat16, both of one type; strided tensors are copied.  z
+    comes from y before it is rounded to that type.
 
     Differentiable in every tensor (once, and not in forward mode: dual tensors are refused).  Up to 16384 channels, with
     gradients in channels_first 4096 (beyond them the forward runs and the backward raises)."""
@@ -315,10 +316,10 @@ def quantize_weight(weight):
 
 
 def int8_product(q, scale, weight_q, weight_scale, bias=None, dtype=torch.float32, data_format="channels_last"):
-    """out[t, n] = (sum_k q[t, k] weight_q[n, k]) scale[t] weight_scale[n] + bias[n] on the tensor cores, the sum exact
-    (K up to 131072) and then rounded to float32.  q (...,K) int8, scale for each of its rows, weight_q (N,K) int8.  The result, float32 or bfloat16,
-    is (...,N), or (B,N,H,W) in channels_first, which takes q as (B,H,W,K).  Rows of q and weight_q that do not begin at
-    multiples of 16 bytes are copied."""
+    """out[t, n] = (sum_k q[t, k] weight_q[n, k]) scale[t] weight_scale[n] + bias[n] on the tensor cores, the sum exact (K up
+    to 131072) and then rounded to float32.  q (...,K) int8, scale for each of its rows, weight_q (N,K) int8.  The result,
+    float32 or bfloat16, is (...,N), or (B,N,H,W) in channels_first, which takes q as (B,H,W,K).  Rows of q and weight_q that
+    do not begin at multiples of 16 bytes are copied."""
     _forward_only("int8_product", scale, weight_scale, bias)
     if dtype not in (torch.float32, torch.bfloat16):
         raise RuntimeError("int8_product gives float32 or bfloat16 tensors, not %s" % dtype)
